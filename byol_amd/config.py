@@ -120,6 +120,10 @@ def build_parser() -> argparse.ArgumentParser:
                              "reference's Apex O2 fp16 experiments")
 
     # MI355X-native knobs (not in the reference)
+    parser.add_argument("--clip-norm", type=float, default=0,
+                        help="bound on the global 2-norm of all gradients "
+                             "(default: 0, no clipping); --clip bounds each "
+                             "value")
     parser.add_argument("--bucket-cap-mb", type=float, default=32.0,
                         help="DDP gradient bucket size in MiB, tuned for "
                              "xGMI (default: 32)")

@@ -9,14 +9,13 @@ import pprint
 import time
 
 import torch
-import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import layers
 from ..data import build_train_and_test_transforms, get_loader
 from ..models.byol import BYOL
 from ..objective import loss_function
-from ..optim import build_optimizer
+from ..optim import build_optimizer, clip_grad_norm_, clip_grad_value_
 from ..parallel import FlatDDP, convert_sync_batchnorm
 from .grapher import Grapher
 from .saver import CheckpointBundle, ModelSaver, get_name
@@ -211,6 +210,14 @@ def execute_graph(epoch, model, loader, grapher, args, optimizer=None,
 
     from ..ops.classifier import cross_entropy_topk
 
+    def clip_gradients():
+        if args.clip > 0:
+            clip_grad_value_(model.parameters(), args.clip)
+        clip_norm = getattr(args, "clip_norm", 0.0)
+        # LAMB clips by norm while it reads the gradients
+        if clip_norm > 0 and not getattr(optimizer, "max_grad_norm", 0.0):
+            clip_grad_norm_(model.parameters(), clip_norm)
+
     def train_step_body(a1, a2, lab):
         """One full training step (fwd + losses + bwd + opt) — runs eager
         or captured into a hipGraph (``--hip-graph``); returns the five
@@ -234,16 +241,14 @@ def execute_graph(epoch, model, loader, grapher, args, optimizer=None,
             if is_ddp:
                 model.finish_grad_sync()
             scaler.unscale_(optimizer)
-            if args.clip > 0:
-                nn.utils.clip_grad_value_(model.parameters(), args.clip)
+            clip_gradients()
             scaler.step(optimizer)
             scaler.update()
         else:
             total.backward()
             if is_ddp:
                 model.finish_grad_sync()
-            if args.clip > 0:
-                nn.utils.clip_grad_value_(model.parameters(), args.clip)
+            clip_gradients()
             optimizer.step()
         if args.polyak_ema > 0:
             layers.polyak_ema_parameters(model, args.polyak_ema)

@@ -49,3 +49,8 @@ def require_extension(what: str):
 
 def has_extension() -> bool:
     return _try_load() is not None
+
+
+from .grad_clip import (clip_grads_by_norm_, clip_grads_by_value_,  # noqa: E402
+                        global_grad_norm)
+from .lamb_step import fused_lamb_step  # noqa: E402

@@ -124,6 +124,8 @@ void launch_lars_momentum_step(float* p, const float* g, float* m,
                                float momentum,
                                int m_init, hipStream_t stream);
 
+void bind_optim(pybind11::module& mod);  // optim_bindings.cpp
+
 namespace {
 
 #define CHECK_IN(t)                                                        \
@@ -574,6 +576,7 @@ void bn_bwd_apply_bf16(torch::Tensor dy, torch::Tensor y, torch::Tensor x,
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
+  bind_optim(mod);
   mod.def("bn_stats_bf16", &bn_stats_bf16);
   mod.def("bn_apply_bf16", &bn_apply_bf16);
   mod.def("bn_bwd_reduce_bf16", &bn_bwd_reduce_bf16);

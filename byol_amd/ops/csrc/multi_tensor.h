@@ -1,0 +1,80 @@
+// Lists of tensors as kernel arguments, for the kernels that pass once over
+// all gradients or parameters of a model (gradclip.hip, lamb.hip).
+//
+// A list travels inside the kernel's own argument block, so a step uploads
+// nothing, keeps nothing between calls, and a captured graph holds its own
+// copy.  The argument block is kept under 4 KB, hence the table sizes; longer
+// lists take several launches.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <vector>
+
+#include "common.h"
+#include "tensor_span.h"
+
+inline int element_size(SpanType type) {
+  return type == SpanType::kF32 ? 4 : 2;
+}
+
+// f(value of the element type): the type of the argument picks the kernel.
+template <typename F>
+void with_element_type(SpanType type, F f) {
+  if (type == SpanType::kF32)
+    f(float());
+  else if (type == SpanType::kBF16)
+    f(__bf16());
+  else
+    f(_Float16());
+}
+
+constexpr int kMaxSpans = 224;
+constexpr int kSpanBlock = 256;
+struct SpanTable {
+  void* ptr[kMaxSpans];
+  uint32_t len[kMaxSpans];
+  int first[kMaxSpans + 1];  // a span's first chunk; [count] = all chunks
+  int count;
+  uint32_t chunk;  // elements
+};
+
+// 16 bytes of elements, loaded and stored as one access at any element
+// alignment (global memory takes unaligned dwordx4 on gfx950).
+template <typename T>
+struct Pack {
+  static constexpr int kLen = 16 / sizeof(T);
+  typedef T type __attribute__((ext_vector_type(16 / sizeof(T)),
+                                aligned(sizeof(T))));
+};
+
+// The span that chunk `c` lies in: spans are in chunk order, so it is the
+// number of spans that begin at or before `c`, less one.  Each lane looks at
+// count/64 entries, which costs one memory latency instead of a search's
+// eight.  All lanes of the wave have to be active.
+__device__ __forceinline__ int span_of_chunk(const int* first, int count,
+                                             int c) {
+  const int lane = threadIdx.x & (WAVE_SIZE - 1);
+  int below = 0;
+  for (int j = 0; j < count; j += WAVE_SIZE) {
+    const int k = j + lane;
+    below += __popcll(__ballot(k < count && first[k] <= c));
+  }
+  return __builtin_amdgcn_readfirstlane(below - 1);
+}
+
+// Block sum in 64 bits, for blocks of kSpanBlock threads; valid in all threads.
+__device__ __forceinline__ double block_sum_f64(double v, double* scratch) {
+  #pragma unroll
+  for (int off = WAVE_SIZE / 2; off > 0; off >>= 1)
+    v += __shfl_xor(v, off, WAVE_SIZE);
+  const int wid = threadIdx.x / WAVE_SIZE;
+  if ((threadIdx.x & (WAVE_SIZE - 1)) == 0) scratch[wid] = v;
+  __syncthreads();
+  double out = scratch[0];
+  #pragma unroll
+  for (int w = 1; w < kSpanBlock / WAVE_SIZE; ++w) out += scratch[w];
+  __syncthreads();
+  return out;
+}

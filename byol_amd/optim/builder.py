@@ -38,7 +38,9 @@ def build_lr_schedule(optimizer, args, last_epoch=-1):
 def build_optimizer(model, args, last_epoch=-1):
     """Returns (optimizer, scheduler).  When the model exposes a flat
     parameter space (``finalize()``d BYOL) the LARS wrapper gets it attached
-    so its step runs as three fused HIP kernel launches on GPU."""
+    so its step runs as three fused HIP kernel launches on GPU; LAMB gets it
+    so its gradients stay in the buffer that FlatDDP reduces.  LAMB clips by
+    ``--clip-norm`` inside its own step."""
     optim_map = {
         "rmsprop": optim.RMSprop,
         "adam": optim.Adam,
@@ -53,9 +55,10 @@ def build_optimizer(model, args, last_epoch=-1):
     is_lars = "lars" in full_opt_name
     if full_opt_name == "lamb":
         # bf16 autocast replaces the reference's fp16-only Apex FusedLAMB
-        # gate; our LAMB is a plain implementation (fused HIP path: TODO).
+        # gate; fp32 parameters on GPU take the fused HIP step
         from .lamb import LAMB
-        optim_map["lamb"] = LAMB
+        optim_map["lamb"] = functools.partial(
+            LAMB, max_grad_norm=getattr(args, "clip_norm", 0.0))
 
     opt_name = full_opt_name.split("_")[-1] if is_lars else full_opt_name
     if opt_name not in optim_map:
@@ -69,8 +72,9 @@ def build_optimizer(model, args, last_epoch=-1):
 
     opt = optim_map[opt_name](params_to_optimize, lr=lr)
 
-    if is_lars:
-        opt = LARS(opt, eps=0.0)
+    if is_lars or opt_name == "lamb":
+        if is_lars:
+            opt = LARS(opt, eps=0.0)
         target = model.module if hasattr(model, "module") else model
         flat_space = getattr(target, "_flat_space", None)
         if flat_space is not None:

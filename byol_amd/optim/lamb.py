@@ -1,20 +1,59 @@
 """LAMB optimizer (replacement for the reference's Apex FusedLAMB,
-``/root/reference/main.py:324-326``).  Plain PyTorch implementation of the
-LAMB update (You et al., arXiv:1904.00962): Adam-style moments, then a
-per-layer trust ratio ``||p|| / ||update||`` scales the step."""
+``/root/reference/main.py:324-326``): the LAMB update (You et al.,
+arXiv:1904.00962) — Adam-style moments, then a per-layer trust ratio
+``||p|| / ||update||`` scales the step.
+
+fp32 parameters on a GPU take the fused step (``byol_amd/ops/lamb_step.py``):
+all tensors in two passes, without a host wait.  Other parameters are updated
+one by one in torch operations.  ``max_grad_norm`` clips the global norm of
+all gradients inside the step, as Apex's optimizer does; the gradients
+themselves are left as they are.
+"""
 
 import torch
 from torch.optim.optimizer import Optimizer
 
 __all__ = ["LAMB"]
 
+_GRAD_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _takes_fused_step(p) -> bool:
+    g = p.grad
+    return (p.is_cuda and p.dtype == torch.float32
+            and g.dtype in _GRAD_DTYPES and g.layout is torch.strided
+            and (p.is_contiguous()
+                 or p.is_contiguous(memory_format=torch.channels_last)))
+
 
 class LAMB(Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-6,
-                 weight_decay=0.0):
+                 weight_decay=0.0, max_grad_norm=0.0):
+        if not max_grad_norm >= 0:
+            raise ValueError(f"invalid max_grad_norm: {max_grad_norm}")
         defaults = dict(lr=lr, betas=betas, eps=eps,
                         weight_decay=weight_decay)
         super().__init__(params, defaults)
+        self.defaults["max_grad_norm"] = float(max_grad_norm)
+
+    @property
+    def max_grad_norm(self) -> float:
+        """Bound on the global gradient norm; 0 means no clipping."""
+        return self.defaults.get("max_grad_norm", 0.0)
+
+    def attach_flat_space(self, flat_space):
+        """Keep gradients as views of the model's flat buffer, which
+        :class:`~byol_amd.parallel.FlatDDP` reduces: ``zero_grad`` then
+        clears them in place instead of dropping them."""
+        flat_space.verify()
+        self._flat_space = flat_space
+
+    def zero_grad(self, set_to_none: bool = True):
+        space = getattr(self, "_flat_space", None)
+        if space is not None:
+            space.zero_grads()
+        else:
+            super().zero_grad(set_to_none=set_to_none)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -22,31 +61,66 @@ class LAMB(Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        norm = None
+        if self.max_grad_norm > 0:
+            from ..ops import global_grad_norm
+            grads = [p.grad for group in self.param_groups
+                     for p in group["params"] if p.grad is not None]
+            if grads:
+                norm = global_grad_norm(grads)
+        fused = {}
         for group in self.param_groups:
-            beta1, beta2 = group["betas"]
+            key = (group["lr"], tuple(group["betas"]), group["eps"])
             for p in group["params"]:
                 if p.grad is None:
                     continue
-                grad = p.grad
                 state = self.state[p]
                 if len(state) == 0:
                     state["step"] = 0
                     state["exp_avg"] = torch.zeros_like(p)
                     state["exp_avg_sq"] = torch.zeros_like(p)
-                exp_avg, exp_avg_sq = state["exp_avg"], state["exp_avg_sq"]
                 state["step"] += 1
-                exp_avg.mul_(beta1).add_(grad, alpha=1 - beta1)
-                exp_avg_sq.mul_(beta2).addcmul_(grad, grad, value=1 - beta2)
-                bias1 = 1 - beta1 ** state["step"]
-                bias2 = 1 - beta2 ** state["step"]
-                update = (exp_avg / bias1) / (
-                    (exp_avg_sq / bias2).sqrt().add_(group["eps"]))
-                if group["weight_decay"] > 0:
-                    update.add_(p, alpha=group["weight_decay"])
-                w_norm = p.norm()
-                u_norm = update.norm()
-                trust = torch.where(
-                    (w_norm > 0) & (u_norm > 0),
-                    w_norm / u_norm, torch.ones_like(w_norm))
-                p.add_(update, alpha=-group["lr"] * float(trust))
+                if not _takes_fused_step(p):
+                    self._step_one(p, state, group, norm)
+                    continue
+                for name in ("exp_avg", "exp_avg_sq"):
+                    # a checkpoint of another memory format
+                    if state[name].stride() != p.stride():
+                        state[name] = torch.empty_like(p).copy_(state[name])
+                lists = fused.setdefault(
+                    (p.device, p.grad.dtype, state["step"], *key),
+                    ([], [], [], [], []))
+                for values, value in zip(lists, (
+                        p, p.grad, state["exp_avg"], state["exp_avg_sq"],
+                        max(group["weight_decay"], 0.0))):
+                    values.append(value)
+        if fused:
+            from ..ops import fused_lamb_step
+            for (_, _, step, lr, betas, eps), lists in fused.items():
+                fused_lamb_step(*lists[:4], step=step, lr=lr, betas=betas,
+                                eps=eps, weight_decay=lists[4],
+                                max_grad_norm=self.max_grad_norm,
+                                grad_norm=norm)
         return loss
+
+    def _step_one(self, p, state, group, norm):
+        beta1, beta2 = group["betas"]
+        grad = p.grad
+        if norm is not None:
+            grad = grad * (self.max_grad_norm / (norm.double() + 1e-6)) \
+                .clamp(max=1.0).to(grad.dtype)
+        exp_avg, exp_avg_sq = state["exp_avg"], state["exp_avg_sq"]
+        exp_avg.mul_(beta1).add_(grad, alpha=1 - beta1)
+        exp_avg_sq.mul_(beta2).addcmul_(grad, grad, value=1 - beta2)
+        bias1 = 1 - beta1 ** state["step"]
+        bias2 = 1 - beta2 ** state["step"]
+        update = (exp_avg / bias1) / (
+            (exp_avg_sq / bias2).sqrt().add_(group["eps"]))
+        if group["weight_decay"] > 0:
+            update.add_(p, alpha=group["weight_decay"])
+        w_norm = p.norm()
+        u_norm = update.norm()
+        trust = torch.where(
+            (w_norm > 0) & (u_norm > 0),
+            w_norm / u_norm, torch.ones_like(w_norm))
+        p.add_(update, alpha=-group["lr"] * float(trust))

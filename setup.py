@@ -25,6 +25,9 @@ sources = [
     os.path.join(CSRC, "conv1x1.hip"),
     os.path.join(CSRC, "conv3x3.hip"),
     os.path.join(CSRC, "bn_bf16.hip"),
+    os.path.join(CSRC, "optim_bindings.cpp"),
+    os.path.join(CSRC, "gradclip.hip"),
+    os.path.join(CSRC, "lamb.hip"),
 ]
 
 setup(
@@ -37,7 +40,10 @@ setup(
             sources=sources,
             extra_compile_args={
                 "cxx": ["-O3"],
-                "nvcc": ["-O3", "-std=c++17"],
+                # packed fp32 instructions stay off: some of their forms
+                # have given wrong results on this hardware
+                "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
+                         "-Xclang", "-packed-fp32-ops"],
             },
         )
     ],

@@ -1,0 +1,397 @@
+"""The fused LAMB step against 64-bit values, its refusals, and the optimizer
+and engine paths that call it.
+
+Tolerances, e = 2^-24 (half an fp32 step), from the step's own operations:
+
+* the clipping factor: the norm is rounded to fp32 (e), so is the factor (e);
+* g' = factor * g: one more rounding, 3e in all;
+* m = b1 m + (1-b1) g': both constants rounded (e each), two products and the
+  sum (e each): e (3 |b1 m| + 6 |(1-b1) g'|);
+* v alike, with g' twice: e (3 b2 v + 11 (1-b2) g'^2) <= 11 e v;
+* u = (m k1) / (sqrt(v k2) + eps) + wd p: with a the first summand, m k1 takes
+  2e, the root (11 + 2) / 2 + 1 e, the sum with a rounded eps 2e, the division
+  e: 13 e |a| beside m's own error; wd p: 2e; the sum e |u|;
+* r = |p| / |u|: |p| is summed in 64 bits; |u| is off by the norm of u's
+  errors; lr r takes 2e (lr and the product rounded);
+* p - lr r u: product and sum, e each.
+
+The CPU form takes its norms from torch in fp32: n e more for n elements, at
+the small sizes where it is tested.  1.01 covers products of these terms.
+"""
+
+import math
+
+import pytest
+import torch
+
+from byol_amd import ops
+from byol_amd.optim.lamb import LAMB
+
+E = 2.0 ** -24
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+B1, B2 = 0.9, 0.999
+
+
+def make(sizes, device, dtype=torch.float32, seed=0, fresh=False, gap=0):
+    """params, grads, exp_avgs, exp_avg_sqs as views of four buffers of
+    sevens, `gap` values between the views."""
+    gen = torch.Generator().manual_seed(seed)
+    total = sum(sizes) + gap * (len(sizes) + 1)
+    arenas = [torch.full((total,), 7.0,
+                         dtype=dtype if k == 1 else torch.float32)
+              for k in range(4)]
+    spans, at = [], gap
+    for i, n in enumerate(sizes):
+        scale = 10.0 ** (-(i % 3))
+        values = [torch.randn(n, generator=gen) * 0.1,
+                  torch.randn(n, generator=gen) * scale,
+                  torch.randn(n, generator=gen) * scale * 0.3,
+                  torch.rand(n, generator=gen) * scale ** 2]
+        if fresh:
+            values[2:] = [torch.zeros(n), torch.zeros(n)]
+        for arena, value in zip(arenas, values):
+            arena[at:at + n] = value
+        spans.append((at, n))
+        at += n + gap
+    arenas = [a.to(device) for a in arenas]
+    return arenas, [[a[s:s + n] for s, n in spans] for a in arenas]
+
+
+def exact(p, g, m, v, step, lr, eps, wd, factor):
+    """The step in 64 bits, and how far p, m and v may be from it."""
+    p, g, m, v = (t.detach().cpu().double() for t in (p, g, m, v))
+    g = g * factor
+    m_old, v_old = m, v
+    m = B1 * m_old + (1 - B1) * g
+    v = B2 * v_old + (1 - B2) * g * g
+    k1 = 1 / (1 - B1 ** step)
+    den = (v / (1 - B2 ** step)).sqrt() + eps
+    a = m * k1 / den
+    u = a + wd * p
+    p_norm, u_norm = p.norm(), u.norm()
+    r = (p_norm / u_norm).item() if p_norm > 0 and u_norm > 0 else 1.0
+    out = p - lr * r * u
+    m_off = E * (3 * (B1 * m_old).abs() + 6 * ((1 - B1) * g).abs())
+    u_off = m_off * k1 / den + E * (13 * a.abs() + 2 * (wd * p).abs()
+                                    + u.abs())
+    r_off = (u_off.norm() / u_norm).item() if r != 1.0 else 0.0
+    p_off = lr * r * (u_off + u.abs() * (r_off + 3 * E)) + E * out.abs()
+    return (out, 1.01 * p_off), (m, 1.01 * m_off), (v, 1.01 * 11 * E * v), \
+        lr * r * u.abs()
+
+
+def check(lists, before, step, lr, eps, decay, factor=1.0, slack=False):
+    for i in range(len(lists[0])):
+        p, m, v, moved = exact(*(b[i] for b in before), step, lr, eps,
+                               decay[i], factor)
+        norm_slack = moved * 2 * moved.numel() * E if slack else 0.0
+        for name, k, (want, off), more in (("p", 0, p, norm_slack),
+                                           ("m", 2, m, 0.0),
+                                           ("v", 3, v, 0.0)):
+            far = (lists[k][i].detach().cpu().double() - want).abs()
+            # 1e-44: results among the subnormal numbers
+            assert (far <= off + more + 1e-44).all(), (name, i,
+                                                       far.max().item())
+
+
+LISTS = {
+    "one value": [1],
+    "one bias": [257],
+    "no values among some": [0, 5, 0, 64],
+    "around a pack": [3, 4, 5, 7, 8, 9],
+    "around a block's share": [4095, 4096, 4097, 8191],
+    "more tensors than a table": [1 + (i * 37) % 300 for i in range(200)],
+}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16,
+                                   torch.float16])
+@pytest.mark.parametrize("step,clip", [(1, 0.0), (1, 0.5), (40, 0.0),
+                                       (3000, 0.5), (3000, 1e6)])
+@pytest.mark.parametrize("sizes", LISTS.values(), ids=LISTS.keys())
+def test_step(device, dtype, step, clip, sizes):
+    arenas, lists = make(sizes, device, dtype, fresh=step == 1, gap=1)
+    before = [[t.clone() for t in ts] for ts in lists]
+    decay = [0.01 * (i % 2) for i in range(len(sizes))]
+    norm = torch.cat([g.cpu().double() for g in before[1]]).norm().item()
+    ops.fused_lamb_step(*lists, step=step, lr=0.1, weight_decay=decay,
+                        max_grad_norm=clip)
+    factor = min(1.0, clip / (norm + 1e-6)) if clip else 1.0
+    check(lists, before, step, 0.1, 1e-6, decay, factor, device == "cpu")
+    for g, b in zip(lists[1], before[1]):
+        assert torch.equal(g, b)
+    edges = sum(1 for _ in sizes) + 1
+    for a in arenas:  # the values between the tensors
+        assert int((a == 7).sum()) >= edges
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [[5_000_001, 3, 700_000],
+                                   [70_000] * 100])
+def test_large_lists(sizes):
+    _, lists = make(sizes, "cuda", gap=1)
+    before = [[t.clone() for t in ts] for ts in lists]
+    decay = [0.01] * len(sizes)
+    ops.fused_lamb_step(*lists, step=7, lr=0.01, weight_decay=decay)
+    check(lists, before, 7, 0.01, 1e-6, decay)
+    again = [[t.clone() for t in ts] for ts in before]
+    ops.fused_lamb_step(*again, step=7, lr=0.01, weight_decay=decay)
+    for a, b in zip(lists, again):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_norms_of_zero(device):
+    """A zero parameter, and one whose update is zero, step with ratio 1."""
+    _, lists = make([300, 300], device)
+    lists[0][0].zero_()
+    for k in (1, 2):
+        lists[k][1].zero_()
+    before = [[t.clone() for t in ts] for ts in lists]
+    ops.fused_lamb_step(*lists, step=2, lr=0.1)
+    check(lists, before, 2, 0.1, 1e-6, [0.0, 0.0], slack=device == "cpu")
+    assert torch.equal(lists[0][1], before[0][1])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_nan_stays_in_its_tensor(device):
+    _, lists = make([300, 300], device)
+    lists[1][0][7] = math.nan
+    before = [[t.clone() for t in ts] for ts in lists]
+    ops.fused_lamb_step(*lists, step=2, lr=0.1)
+    assert lists[0][0][7].isnan() and lists[2][0][7].isnan()
+    assert int(lists[0][0].isnan().sum()) == 1
+    check([t[1:] for t in lists], [b[1:] for b in before], 2, 0.1, 1e-6,
+          [0.0], slack=device == "cpu")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layouts(device):
+    """Channels-last parameters, and gradients laid out unlike them."""
+    torch.manual_seed(0)
+    shapes = [(8, 6, 3, 3), (8, 6, 1, 1), (5, 40)]
+    def like():
+        return [torch.rand(shapes[0]).to(memory_format=torch.channels_last),
+                torch.rand(shapes[1]), torch.rand(shapes[2]).t()]
+    lists = [[t.to(device) for t in like()] for _ in range(4)]
+    lists[1] = [g.contiguous() for g in lists[1]]
+    lists[1][1] = lists[1][1].to(memory_format=torch.channels_last)
+    before = [[t.clone() for t in ts] for ts in lists]
+    ops.fused_lamb_step(*lists, step=3, lr=0.1, weight_decay=0.01)
+    check(lists, before, 3, 0.1, 1e-6, [0.01] * 3, slack=device == "cpu")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    _, (p, g, m, v) = make([64, 8], device)
+    before = [t.clone() for t in p + m + v]
+    for bad in (dict(step=0), dict(step=1, betas=(1.0, 0.9)),
+                dict(step=1, betas=(0.9, -0.1)), dict(step=1, eps=-1.0),
+                dict(step=1, max_grad_norm=-1.0),
+                dict(step=1, max_grad_norm=math.nan),
+                dict(step=1, weight_decay=[0.1])):
+        with pytest.raises(ValueError):
+            ops.fused_lamb_step(p, g, m, v, lr=0.1, **bad)
+    with pytest.raises(ValueError):
+        ops.fused_lamb_step(p, g, m[:1], v, step=1, lr=0.1)
+    with pytest.raises(ValueError, match="shape"):
+        ops.fused_lamb_step(p, [g[0], g[0]], m, v, step=1, lr=0.1)
+    with pytest.raises(TypeError):
+        ops.fused_lamb_step([t.double() for t in p], g, m, v, step=1, lr=0.1)
+    with pytest.raises(TypeError):
+        ops.fused_lamb_step(p, g, [t.half() for t in m], v, step=1, lr=0.1)
+    for a, b in zip(p + m + v, before):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.skipif(not ops.has_extension(), reason="extension not built")
+def test_binding_refuses_before_any_launch():
+    """The checks of the binding itself, on CPU tensors: it never launches
+    for them."""
+    ext = ops.extension()
+
+    def call(p, g, m, v, step=1, norm=None):
+        ext.lamb_step(p, g, m, v, [0.0] * len(p), step, 0.1, B1, B2, 1e-6,
+                      1.0, norm)
+
+    _, (p, g, m, v) = make([64, 8], "cpu")
+    sides = torch.rand(8, 8)
+    for bad, text in (
+            ((p, g, m, v), "GPU"),
+            ((p, g, m, v, 0), "step"),
+            ((p, g, m, m), "twice"),
+            ((p, g, p, v), "twice"),
+            (([p[0], p[0]], [g[0]] * 2, m, v), "strides|twice"),
+            ((p, p, m, v), "gradient shares memory"),
+            ((p, g, m, [v[1], v[0]]), "strides"),
+            (([sides], [sides.clone()], [sides.t().clone(
+                memory_format=torch.preserve_format)],
+              [torch.rand(8, 8)]), "strides"),
+            (([p[0][::2]], [g[0][::2]], [m[0][::2]], [v[0][::2]]), "dense"),
+            ((p, g[::-1], m, v), "shape")):
+        with pytest.raises(ValueError, match=text):
+            call(*bad)
+    for bad in (([t.double() for t in p], g, m, v),
+                (p, [t.double() for t in g], m, v),
+                (p, [g[0], g[1].half()], m, v)):
+        with pytest.raises(TypeError):
+            call(*bad)
+
+
+def small_model(device, seed=0):
+    torch.manual_seed(seed)
+    return torch.nn.Sequential(
+        torch.nn.Conv2d(3, 8, 3), torch.nn.BatchNorm2d(8), torch.nn.ReLU(),
+        torch.nn.Flatten(), torch.nn.Linear(8 * 36, 5)).to(device)
+
+
+def train(model, opt, steps=4, seed=3):
+    gen = torch.Generator().manual_seed(seed)
+    device = next(model.parameters()).device
+    for _ in range(steps):
+        opt.zero_grad()
+        x = torch.randn(16, 3, 8, 8, generator=gen).to(device)
+        model(x).square().mean().backward()
+        opt.step()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_optimizer_clips_like_clipping_first(device):
+    """max_grad_norm inside the step is clipping the gradients before it:
+    alike within a rounding of each gradient."""
+    from byol_amd.optim import clip_grad_norm_
+    grads = [torch.randn(40, 9), torch.randn(9)]
+    results = []
+    for inside in (True, False):
+        params = [torch.nn.Parameter((torch.ones(g.shape) * 0.1).to(device))
+                  for g in grads]
+        opt = LAMB(params, lr=0.1, weight_decay=0.01,
+                   max_grad_norm=0.25 if inside else 0.0)
+        assert opt.max_grad_norm == (0.25 if inside else 0.0)
+        for p, g in zip(params, grads):
+            p.grad = g.to(device)
+        if not inside:
+            clip_grad_norm_(params, 0.25)
+        opt.step()
+        results.append(params)
+    # the first step's update is g' / (|g'| + eps) in each element
+    for a, b in zip(*results):
+        assert torch.allclose(a, b, rtol=16 * E, atol=16 * E * 0.1)
+
+
+@pytest.mark.gpu
+def test_optimizer_matches_its_cpu_form():
+    """One step from the same gradients; then state dicts move between the
+    devices and the next step still agrees."""
+    cpu, gpu = small_model("cpu"), small_model("cuda")
+    groups = [[{"params": [p for p in m.parameters() if p.ndim > 1],
+                "weight_decay": 0.01},
+               {"params": [p for p in m.parameters() if p.ndim <= 1],
+                "weight_decay": 0.0}] for m in (cpu, gpu)]
+    opts = [LAMB(g, lr=0.05, max_grad_norm=1.0) for g in groups]
+    gen = torch.Generator().manual_seed(1)
+    for turn in range(3):
+        for p, q in zip(cpu.parameters(), gpu.parameters()):
+            q.data.copy_(p.data)
+            p.grad = torch.randn(p.shape, generator=gen)
+            q.grad = p.grad.to("cuda")
+        for o in opts:
+            o.step()
+        for p, q in zip(cpu.parameters(), gpu.parameters()):
+            # the steps' own bounds, doubled for two forms; sums of up to
+            # 1440 elements in fp32 on the CPU
+            far = (q.detach().cpu() - p.detach()).abs()
+            assert (far <= 2 * (p.detach().abs() * E
+                                + 0.05 * p.detach().norm()
+                                * (40 + p.numel()) * E)).all()
+        opts[1].load_state_dict(opts[0].state_dict())
+    assert opts[1].state[next(gpu.parameters())]["step"] == 3
+
+
+@pytest.mark.gpu
+def test_optimizer_mixes_fused_and_single_parameters():
+    """A bf16 and a sliced parameter beside fp32 ones: each is stepped."""
+    torch.manual_seed(0)
+    base = torch.randn(10, 8, device="cuda")
+    params = [torch.nn.Parameter(torch.randn(33, device="cuda")),
+              torch.nn.Parameter(torch.randn(12, device="cuda").bfloat16()),
+              torch.nn.Parameter(base[:, ::2])]
+    before = [p.detach().clone() for p in params]
+    opt = LAMB(params, lr=0.1, max_grad_norm=10.0)
+    for p in params:
+        p.grad = torch.randn_like(p)
+    opt.step()
+    for p, b in zip(params, before):
+        assert torch.isfinite(p).all() and not torch.equal(p, b)
+        assert opt.state[p]["step"] == 1
+
+
+@pytest.mark.gpu
+def test_step_refuses_capture():
+    _, lists = make([64], "cuda")
+    before = lists[0][0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="captured"):
+            ops.fused_lamb_step(*lists, step=1, lr=0.1)
+        lists[1][0].mul_(1.0)
+    torch.cuda.synchronize()
+    assert torch.equal(lists[0][0], before)
+
+
+@pytest.mark.gpu
+def test_two_streams():
+    made = [make([300_001, 50], "cuda", seed=s, gap=1)[1] for s in (1, 2)]
+    before = [[[t.clone() for t in ts] for ts in lists] for lists in made]
+    streams = [torch.cuda.Stream() for _ in made]
+    torch.cuda.synchronize()
+    for lists, s in zip(made, streams):
+        with torch.cuda.stream(s):
+            ops.fused_lamb_step(*lists, step=5, lr=0.1, max_grad_norm=1.0)
+    torch.cuda.synchronize()
+    for lists, b in zip(made, before):
+        norm = torch.cat([g.cpu().double() for g in b[1]]).norm().item()
+        check(lists, b, 5, 0.1, 1e-6, [0.0, 0.0], 1.0 / (norm + 1e-6))
+
+
+def engine_args(tmp_path, device, *extra):
+    import byol_amd.config as config
+    args = config.parse_args([
+        "--task", "synthetic_multi_augment_image_folder",
+        "--arch", "resnet18", "--representation-size", "512",
+        "--head-latent-size", "64", "--projection-size", "32",
+        "--batch-size", "8", "--epochs", "1", "--num-replicas", "1",
+        "--image-size-override", "32", "--synthetic-classes", "8",
+        "--synthetic-train-samples", "32", "--synthetic-test-samples", "8",
+        "--workers-per-replica", "0", "--model-dir", str(tmp_path / "m"),
+        "--log-dir", str(tmp_path / "l"), *extra])
+    args.cuda = device == "cuda"
+    args.distributed_rank = 0
+    return args
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("extra", [
+    ("--optimizer", "lamb", "--lr", "0.001", "--clip-norm", "1.0"),
+    ("--clip-norm", "1.0", "--clip", "0.5")])
+def test_engine_epoch(device, extra, tmp_path):
+    """Norm, clipping and step together, as the training engine runs them."""
+    from byol_amd.engine import trainer
+    from byol_amd.optim import build_optimizer
+    args = engine_args(tmp_path, device, *extra)
+    torch.manual_seed(0)
+    loader, model, grapher = trainer.build_loader_model_grapher(args)
+    opt, _ = build_optimizer(model, args)
+    for group in opt.param_groups:
+        group["lr"] = 0.001  # past the warmup's zero
+    before = model.flat_space.flat_params.clone()
+    trainer.train(1, model, opt, loader.train_loader, grapher, args)
+    flat = model.flat_space.flat_params
+    assert torch.isfinite(flat).all() and not torch.equal(flat, before)
+    if "lamb" in extra:
+        assert opt.max_grad_norm == 1.0
+        assert {s["step"] for s in opt.state.values()} == {4}
+        # the gradients live in the flat buffer still
+        model.flat_space.flat_grads.fill_(2.0)
+        assert all((p.grad == 2).all() for p in model.parameters())
