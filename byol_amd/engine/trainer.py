@@ -252,7 +252,11 @@ def execute_graph(epoch, model, loader, grapher, args, optimizer=None,
             optimizer.step()
         if args.polyak_ema > 0:
             layers.polyak_ema_parameters(model, args.polyak_ema)
-        return total, byol_loss, classifier_loss, acc1, acc5
+        # detached: a loss that lives on keeps its step's autograd graph, and
+        # a backward pass captured while an eager graph of the same
+        # parameters lives ends the process
+        return (total.detach(), byol_loss.detach(), classifier_loss.detach(),
+                acc1, acc5)
 
     # hipGraph path: single-GPU training without polyak (the graph wrapper
     # owns the EMA decay/LR device scalars; DDP+graph is a later

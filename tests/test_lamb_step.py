@@ -374,7 +374,8 @@ def engine_args(tmp_path, device, *extra):
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("extra", [
     ("--optimizer", "lamb", "--lr", "0.001", "--clip-norm", "1.0"),
-    ("--clip-norm", "1.0", "--clip", "0.5")])
+    ("--clip-norm", "1.0", "--clip", "0.5"),
+    ("--clip-norm", "1.0", "--channels-last", "--hip-graph")])
 def test_engine_epoch(device, extra, tmp_path):
     """Norm, clipping and step together, as the training engine runs them."""
     from byol_amd.engine import trainer
