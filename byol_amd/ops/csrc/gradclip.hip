@@ -11,7 +11,9 @@
 // pass stays bound by memory (two 64-bit operations for four bytes).
 #include "multi_tensor.h"
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -20,40 +22,80 @@ __device__ __forceinline__ uint32_t magnitude_bits(float x) {
   return __float_as_uint(x) & 0x7fffffffu;
 }
 
+// Four running results each, so that one value's operation does not wait for
+// the one before it.
 struct SumOfSquares {
-  double acc = 0.0;
-  __device__ __forceinline__ void add(float x) {
+  double acc[4] = {0.0, 0.0, 0.0, 0.0};
+  __device__ __forceinline__ void add(float x, int j) {
     const double d = x;
-    acc = fma(d, d, acc);
+    acc[j & 3] = fma(d, d, acc[j & 3]);
   }
+  __device__ __forceinline__ void merge(double sum, int j) {
+    acc[j & 3] += sum;
+  }
+  template <int kThreads>
   __device__ __forceinline__ double join(double* scratch) {
-    return block_sum_f64(acc, scratch);
+    return block_sum_f64<kThreads>((acc[0] + acc[1]) + (acc[2] + acc[3]),
+                                   scratch);
+  }
+  static __device__ __forceinline__ double norm(double sum) {
+    return sqrt(sum);
   }
 };
 
 struct LargestMagnitude {
-  uint32_t acc = 0;
-  __device__ __forceinline__ void add(float x) {
-    const uint32_t b = magnitude_bits(x);
-    acc = b > acc ? b : acc;
+  uint32_t acc[4] = {0, 0, 0, 0};
+  __device__ __forceinline__ void add(float x, int j) {
+    acc[j & 3] = max(acc[j & 3], magnitude_bits(x));
   }
+  __device__ __forceinline__ void merge(double largest, int j) {
+    add(static_cast<float>(largest), j);
+  }
+  template <int kThreads>
   __device__ __forceinline__ double join(double* scratch) {
-    uint32_t v = acc;
+    uint32_t v = max(max(acc[0], acc[1]), max(acc[2], acc[3]));
     #pragma unroll
-    for (int off = WAVE_SIZE / 2; off > 0; off >>= 1) {
-      const uint32_t o = __shfl_xor(v, off, WAVE_SIZE);
-      v = o > v ? o : v;
-    }
+    for (int off = WAVE_SIZE / 2; off > 0; off >>= 1)
+      v = max(v, static_cast<uint32_t>(__shfl_xor(v, off, WAVE_SIZE)));
     uint32_t* s = reinterpret_cast<uint32_t*>(scratch);
     if ((threadIdx.x & (WAVE_SIZE - 1)) == 0) s[threadIdx.x / WAVE_SIZE] = v;
     __syncthreads();
     v = s[0];
     #pragma unroll
-    for (int w = 1; w < kSpanBlock / WAVE_SIZE; ++w) v = s[w] > v ? s[w] : v;
+    for (int w = 1; w < kThreads / WAVE_SIZE; ++w) v = max(v, s[w]);
     __syncthreads();
     return static_cast<double>(__uint_as_float(v));
   }
+  static __device__ __forceinline__ double norm(double largest) {
+    return largest;
+  }
 };
+
+// The part of a span that one block works on.
+template <typename T>
+struct Chunk {
+  T* data;
+  uint32_t packs, n;  // whole packs, elements
+
+  __device__ __forceinline__ Chunk(const SpanTable& table, int c) {
+    const int s = span_of_chunk(table.first, table.count, c);
+    const uint32_t begin = uint32_t(c - table.first[s]) * table.chunk;
+    const uint32_t left = table.len[s] - begin;
+    n = left < table.chunk ? left : table.chunk;
+    packs = n / Pack<T>::kLen;
+    data = static_cast<T*>(table.ptr[s]) + begin;
+  }
+};
+
+// Above this size a list does not stay in the 256 MB memory-side cache
+// between two steps.
+constexpr int64_t kCachedBytes = 128 << 20;
+
+// Loads of a thread in flight at a time.
+constexpr int kUnroll = 4;
+
+// The single block that joins all partial results.
+constexpr int kJoinBlock = 1024;
 
 template <typename T, typename Reduce>
 __global__ __launch_bounds__(kSpanBlock) void grad_norm_partial_kernel(
@@ -61,145 +103,192 @@ __global__ __launch_bounds__(kSpanBlock) void grad_norm_partial_kernel(
   __shared__ double scratch[kSpanBlock / WAVE_SIZE];
   using V = typename Pack<T>::type;
   constexpr int L = Pack<T>::kLen;
-  const int c = blockIdx.x;
-  const int s = span_of_chunk(table.first, table.count, c);
-  const uint32_t begin = uint32_t(c - table.first[s]) * table.chunk;
-  const uint32_t left = table.len[s] - begin;
-  const uint32_t n = left < table.chunk ? left : table.chunk;
-  const T* g = static_cast<const T*>(table.ptr[s]) + begin;
-  const V* gv = reinterpret_cast<const V*>(g);
-  const uint32_t nv = n / L;
+  const Chunk<const T> chunk(table, blockIdx.x);
+  const V* packs = reinterpret_cast<const V*>(chunk.data);
   Reduce red;
-  for (uint32_t i = threadIdx.x; i < nv; i += kSpanBlock) {
-    const V v = gv[i];
+  auto add = [&](const V& v) {
     #pragma unroll
-    for (int j = 0; j < L; ++j) red.add(static_cast<float>(v[j]));
+    for (int j = 0; j < L; ++j) red.add(static_cast<float>(v[j]), j);
+  };
+  uint32_t i = threadIdx.x;
+  for (; i + (kUnroll - 1) * kSpanBlock < chunk.packs;
+       i += kUnroll * kSpanBlock) {
+    V v[kUnroll];
+    #pragma unroll
+    for (int k = 0; k < kUnroll; ++k) v[k] = packs[i + k * kSpanBlock];
+    #pragma unroll
+    for (int k = 0; k < kUnroll; ++k) add(v[k]);
   }
-  const uint32_t t = nv * L + threadIdx.x;
-  if (t < n) red.add(static_cast<float>(g[t]));
-  const double sum = red.join(scratch);
-  if (threadIdx.x == 0) partial[c] = sum;
+  for (; i < chunk.packs; i += kSpanBlock) add(packs[i]);
+  const uint32_t t = chunk.packs * L + threadIdx.x;
+  if (t < chunk.n) red.add(static_cast<float>(chunk.data[t]), 0);
+  const double sum = red.template join<kSpanBlock>(scratch);
+  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-// out[0] = norm, out[1] = the factor for a bound (if bound >= 0)
-template <bool kInf>
-__global__ __launch_bounds__(kSpanBlock) void grad_norm_finish_kernel(
-    const double* __restrict__ partial, int n, double bound,
-    float* __restrict__ out) {
-  __shared__ double scratch[kSpanBlock / WAVE_SIZE];
-  double norm;
-  if (kInf) {
-    LargestMagnitude red;
-    for (int i = threadIdx.x; i < n; i += kSpanBlock)
-      red.add(static_cast<float>(partial[i]));
-    norm = red.join(scratch);
-  } else {
-    double acc = 0.0;
-    for (int i = threadIdx.x; i < n; i += kSpanBlock) acc += partial[i];
-    norm = sqrt(block_sum_f64(acc, scratch));
+// Joins partial results in a fixed order, for blocks of kThreads; the sum of
+// squares or the largest magnitude, in all threads.
+template <typename Reduce, int kThreads>
+__device__ __forceinline__ double join_partials(
+    const double* __restrict__ partial, int n, double* scratch) {
+  Reduce red;
+  int i = threadIdx.x;
+  for (; i + 3 * kThreads < n; i += 4 * kThreads) {
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) red.merge(partial[i + k * kThreads], k);
   }
-  if (threadIdx.x == 0) {
-    out[0] = static_cast<float>(norm);
-    const double c = bound / (norm + 1e-6);
-    out[1] = c >= 1.0 ? 1.f : static_cast<float>(c);  // NaN stays
-  }
+  for (; i < n; i += kThreads) red.merge(partial[i], 0);
+  return red.template join<kThreads>(scratch);
+}
+
+// One block: the norm, or (for a scaling pass over many tables) one partial
+// result in the place of many.
+template <typename Reduce>
+__global__ __launch_bounds__(kJoinBlock) void grad_norm_finish_kernel(
+    const double* __restrict__ partial, int n, float* __restrict__ norm,
+    double* __restrict__ joined) {
+  __shared__ double scratch[kJoinBlock / WAVE_SIZE];
+  const double all = join_partials<Reduce, kJoinBlock>(partial, n, scratch);
+  if (threadIdx.x != 0) return;
+  if (joined != nullptr)
+    *joined = all;
+  else
+    *norm = static_cast<float>(Reduce::norm(all));
 }
 
 // Both clipping passes: `f` maps one value.
-template <typename T, typename F>
-__device__ __forceinline__ void map_chunk(const SpanTable& table, F f) {
+template <typename T, bool kStream, typename F>
+__device__ __forceinline__ void map_chunk(const Chunk<T>& chunk, F f) {
   using V = typename Pack<T>::type;
   constexpr int L = Pack<T>::kLen;
-  const int c = blockIdx.x;
-  const int s = span_of_chunk(table.first, table.count, c);
-  const uint32_t begin = uint32_t(c - table.first[s]) * table.chunk;
-  const uint32_t left = table.len[s] - begin;
-  const uint32_t n = left < table.chunk ? left : table.chunk;
-  T* g = static_cast<T*>(table.ptr[s]) + begin;
-  V* gv = reinterpret_cast<V*>(g);
-  const uint32_t nv = n / L;
-  for (uint32_t i = threadIdx.x; i < nv; i += kSpanBlock) {
-    V v = gv[i];
+  V* packs = reinterpret_cast<V*>(chunk.data);
+  auto map = [&](V v) {
     #pragma unroll
     for (int j = 0; j < L; ++j)
       v[j] = static_cast<T>(f(static_cast<float>(v[j])));
-    gv[i] = v;
+    return v;
+  };
+  uint32_t i = threadIdx.x;
+  for (; i + (kUnroll - 1) * kSpanBlock < chunk.packs;
+       i += kUnroll * kSpanBlock) {
+    V v[kUnroll];
+    #pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      V* at = packs + i + k * kSpanBlock;
+      v[k] = kStream ? __builtin_nontemporal_load(at) : *at;
+    }
+    #pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      V* at = packs + i + k * kSpanBlock;
+      if (kStream)
+        __builtin_nontemporal_store(map(v[k]), at);
+      else
+        *at = map(v[k]);
+    }
   }
-  const uint32_t t = nv * L + threadIdx.x;
-  if (t < n) g[t] = static_cast<T>(f(static_cast<float>(g[t])));
+  for (; i < chunk.packs; i += kSpanBlock) packs[i] = map(packs[i]);
+  const uint32_t t = chunk.packs * L + threadIdx.x;
+  if (t < chunk.n)
+    chunk.data[t] = static_cast<T>(f(static_cast<float>(chunk.data[t])));
 }
 
-template <typename T>
+template <typename T, typename Reduce>
 __global__ __launch_bounds__(kSpanBlock) void grad_scale_kernel(
-    const SpanTable table, const float* __restrict__ factor) {
-  const float c = *factor;
-  if (c == 1.f) return;  // nothing to clip
-  map_chunk<T>(table, [c](float x) { return c * x; });
+    const SpanTable table, const double* __restrict__ partial, int n,
+    double bound, float* __restrict__ norm_out) {
+  __shared__ double scratch[kSpanBlock / WAVE_SIZE];
+  const double norm =
+      Reduce::norm(join_partials<Reduce, kSpanBlock>(partial, n, scratch));
+  if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0)
+    *norm_out = static_cast<float>(norm);
+  const double ratio = bound / (norm + 1e-6);
+  if (ratio >= 1.0) return;  // not for NaN
+  const float f = static_cast<float>(ratio);
+  const int c = mirrored_chunk();
+  if (f == 1.f || c >= table.first[table.count]) return;
+  map_chunk<T, true>(Chunk<T>(table, c), [f](float x) { return f * x; });
 }
 
-template <typename T>
+template <typename T, bool kStream>
 __global__ __launch_bounds__(kSpanBlock) void grad_clamp_kernel(
     const SpanTable table, float bound) {
   // comparisons with NaN are false, so NaN stays
-  map_chunk<T>(table, [bound](float x) {
+  map_chunk<T, kStream>(Chunk<T>(table, blockIdx.x), [bound](float x) {
     return x > bound ? bound : x < -bound ? -bound : x;
   });
 }
 
-// Elements of a chunk, the same for all launches of one call.
-int64_t chunk_elements(const std::vector<TensorSpan>& spans, int elem) {
-  int64_t total = 0;
-  for (const TensorSpan& s : spans) total += s.len;
-  const int64_t step = kSpanBlock * (16 / elem);
-  const int64_t want = (total + 2047) / 2048;
-  const int64_t least = 2 * step;
-  const int64_t chunk = (want + step - 1) / step * step;
-  const int64_t most = kMaxSpanLen;
-  return chunk < least ? least : chunk > most ? most : chunk;
+// A table's chunk, in elements: about kTableChunks chunks, but no less than
+// two packs for each thread.
+int64_t chunk_elements(int64_t total, SpanType type) {
+  const int64_t step = kSpanBlock * (16 / element_size(type));
+  const int64_t want = (total + kTableChunks - 1) / kTableChunks;
+  return std::max(2 * step, (want + step - 1) / step * step);
 }
 
-// Calls `launch(table, chunks, chunks of the launches before)` for as many
-// tables as the list takes; returns the number of chunks.
-template <typename Launch>
-int for_tables(const std::vector<TensorSpan>& spans, int64_t chunk,
-               Launch launch) {
-  SpanTable table;
-  table.chunk = static_cast<uint32_t>(chunk);
-  table.count = 0;
-  table.first[0] = 0;
-  int done = 0;
-  auto flush = [&]() {
-    if (table.count == 0) return;
+// The list in tables of at most kMaxSpans; calls f(table, chunks, chunks of
+// the tables before) for each and returns the number of all chunks.
+template <typename F>
+int64_t for_tables(const std::vector<TensorSpan>& spans, SpanType type, F f) {
+  int64_t done = 0;
+  for (size_t at = 0; at < spans.size(); at += kMaxSpans) {
+    SpanTable table;
+    table.count =
+        static_cast<int>(std::min<size_t>(kMaxSpans, spans.size() - at));
+    int64_t total = 0;
+    for (int i = 0; i < table.count; ++i) total += spans[at + i].len;
+    const int64_t chunk = chunk_elements(total, type);
+    table.chunk = static_cast<uint32_t>(chunk);
+    table.first[0] = 0;
+    for (int i = 0; i < table.count; ++i) {
+      const TensorSpan& s = spans[at + i];
+      table.ptr[i] = s.ptr;
+      table.len[i] = static_cast<uint32_t>(s.len);
+      table.first[i + 1] =
+          table.first[i] + static_cast<int>((s.len + chunk - 1) / chunk);
+    }
     const int chunks = table.first[table.count];
-    launch(table, chunks, done);
+    f(table, chunks, done);
     done += chunks;
-    table.count = 0;
-  };
-  for (const TensorSpan& s : spans) {
-    const int at = table.count++;
-    table.ptr[at] = s.ptr;
-    table.len[at] = static_cast<uint32_t>(s.len);
-    table.first[at + 1] =
-        table.first[at] + static_cast<int>((s.len + chunk - 1) / chunk);
-    if (table.count == kMaxSpans) flush();
   }
-  flush();
   return done;
 }
 
 template <typename Reduce>
-int launch_partials(const std::vector<TensorSpan>& spans, SpanType type,
-                    double* partial, hipStream_t stream) {
-  return for_tables(
-      spans, chunk_elements(spans, element_size(type)),
-      [&](const SpanTable& t, int chunks, int done) {
-        with_element_type(type, [&](auto value) {
-          using T = decltype(value);
-          hipLaunchKernelGGL((grad_norm_partial_kernel<T, Reduce>),
-                             dim3(chunks), dim3(kSpanBlock), 0, stream, t,
-                             partial + done);
-        });
-      });
+int64_t launch_partials(const std::vector<TensorSpan>& spans, SpanType type,
+                        double* partial, hipStream_t stream) {
+  return for_tables(spans, type, [&](const SpanTable& t, int chunks,
+                                     int64_t done) {
+    with_element_type(type, [&](auto value) {
+      hipLaunchKernelGGL(
+          (grad_norm_partial_kernel<decltype(value), Reduce>), dim3(chunks),
+          dim3(kSpanBlock), 0, stream, t, partial + done);
+    });
+  });
+}
+
+template <typename Reduce>
+void launch_scale(const std::vector<TensorSpan>& spans, SpanType type,
+                  const double* partial, int n, double bound, float* norm,
+                  hipStream_t stream) {
+  for_tables(spans, type, [&](const SpanTable& t, int chunks, int64_t done) {
+    with_element_type(type, [&](auto value) {
+      hipLaunchKernelGGL((grad_scale_kernel<decltype(value), Reduce>),
+                         dim3((chunks + 7) / 8 * 8), dim3(kSpanBlock), 0,
+                         stream, t, partial, n, bound,
+                         done == 0 ? norm : nullptr);
+    });
+  });
+}
+
+void launch_finish(const double* partial, int n, bool inf, float* norm,
+                   double* joined, hipStream_t stream) {
+  if (inf)
+    hipLaunchKernelGGL((grad_norm_finish_kernel<LargestMagnitude>), dim3(1),
+                       dim3(kJoinBlock), 0, stream, partial, n, norm, joined);
+  else
+    hipLaunchKernelGGL((grad_norm_finish_kernel<SumOfSquares>), dim3(1),
+                       dim3(kJoinBlock), 0, stream, partial, n, norm, joined);
 }
 
 }  // namespace
@@ -207,51 +296,52 @@ int launch_partials(const std::vector<TensorSpan>& spans, SpanType type,
 // Partial results that launch_grad_norm_partial writes for this list.
 int64_t grad_norm_partials(const std::vector<TensorSpan>& spans,
                            SpanType type) {
-  const int64_t chunk = chunk_elements(spans, element_size(type));
-  int64_t n = 0;
-  for (const TensorSpan& s : spans) n += (s.len + chunk - 1) / chunk;
-  return n;
+  return for_tables(spans, type, [](const SpanTable&, int, int64_t) {});
 }
 
-void launch_grad_norm_partial(const std::vector<TensorSpan>& spans,
-                              SpanType type, bool inf, double* partial,
-                              hipStream_t stream) {
-  if (inf)
-    launch_partials<LargestMagnitude>(spans, type, partial, stream);
-  else
-    launch_partials<SumOfSquares>(spans, type, partial, stream);
+int64_t launch_grad_norm_partial(const std::vector<TensorSpan>& spans,
+                                 SpanType type, bool inf, double* partial,
+                                 hipStream_t stream) {
+  return inf ? launch_partials<LargestMagnitude>(spans, type, partial, stream)
+             : launch_partials<SumOfSquares>(spans, type, partial, stream);
 }
 
 void launch_grad_norm_finish(const double* partial, int64_t n, bool inf,
-                             double bound, float* out, hipStream_t stream) {
-  if (inf)
-    hipLaunchKernelGGL((grad_norm_finish_kernel<true>), dim3(1),
-                       dim3(kSpanBlock), 0, stream, partial, (int)n, bound,
-                       out);
-  else
-    hipLaunchKernelGGL((grad_norm_finish_kernel<false>), dim3(1),
-                       dim3(kSpanBlock), 0, stream, partial, (int)n, bound,
-                       out);
+                             float* norm, hipStream_t stream) {
+  launch_finish(partial, static_cast<int>(n), inf, norm, nullptr, stream);
+}
+
+void launch_grad_norm_join(const double* partial, int64_t n, bool inf,
+                           double* joined, hipStream_t stream) {
+  launch_finish(partial, static_cast<int>(n), inf, nullptr, joined, stream);
 }
 
 void launch_grad_scale(const std::vector<TensorSpan>& spans, SpanType type,
-                       const float* factor, hipStream_t stream) {
-  for_tables(spans, chunk_elements(spans, element_size(type)),
-             [&](const SpanTable& t, int chunks, int) {
-    with_element_type(type, [&](auto value) {
-      hipLaunchKernelGGL((grad_scale_kernel<decltype(value)>), dim3(chunks),
-                         dim3(kSpanBlock), 0, stream, t, factor);
-    });
-  });
+                       bool inf, const double* partial, int64_t n,
+                       double bound, float* norm, hipStream_t stream) {
+  if (inf)
+    launch_scale<LargestMagnitude>(spans, type, partial, static_cast<int>(n),
+                                   bound, norm, stream);
+  else
+    launch_scale<SumOfSquares>(spans, type, partial, static_cast<int>(n),
+                               bound, norm, stream);
 }
 
 void launch_grad_clamp(const std::vector<TensorSpan>& spans, SpanType type,
                        float bound, hipStream_t stream) {
-  for_tables(spans, chunk_elements(spans, element_size(type)),
-             [&](const SpanTable& t, int chunks, int) {
+  int64_t total = 0;
+  for (const TensorSpan& s : spans) total += s.len;
+  const bool streamed = total * element_size(type) > kCachedBytes;
+  for_tables(spans, type, [&](const SpanTable& t, int chunks, int64_t) {
     with_element_type(type, [&](auto value) {
-      hipLaunchKernelGGL((grad_clamp_kernel<decltype(value)>), dim3(chunks),
-                         dim3(kSpanBlock), 0, stream, t, bound);
+      using T = decltype(value);
+      const dim3 grid(chunks), block(kSpanBlock);
+      if (streamed)
+        hipLaunchKernelGGL((grad_clamp_kernel<T, true>), grid, block, 0,
+                           stream, t, bound);
+      else
+        hipLaunchKernelGGL((grad_clamp_kernel<T, false>), grid, block, 0,
+                           stream, t, bound);
     });
   });
 }

@@ -80,7 +80,8 @@ __global__ __launch_bounds__(kSpanBlock) void lamb_moments_kernel(
   const uint32_t nv = n / 4;
   for (uint32_t i = threadIdx.x; i < nv; i += kSpanBlock) {
     const V pv = reinterpret_cast<const V*>(p)[i];
-    const VG gv = reinterpret_cast<const VG*>(g)[i];
+    const VG gv =
+        __builtin_nontemporal_load(reinterpret_cast<const VG*>(g) + i);
     V mv = reinterpret_cast<const V*>(m)[i];
     V vv = reinterpret_cast<const V*>(v)[i];
     #pragma unroll
@@ -100,8 +101,8 @@ __global__ __launch_bounds__(kSpanBlock) void lamb_moments_kernel(
     m[t] = mj;
     v[t] = vj;
   }
-  const double psum = block_sum_f64(pp, scratch);
-  const double usum = block_sum_f64(uu, scratch);
+  const double psum = block_sum_f64<kSpanBlock>(pp, scratch);
+  const double usum = block_sum_f64<kSpanBlock>(uu, scratch);
   if (threadIdx.x == 0) sums[c] = make_double2(psum, usum);
 }
 
@@ -109,7 +110,8 @@ __global__ __launch_bounds__(kSpanBlock) void lamb_update_kernel(
     const LambTable table, LambRates r, const double2* __restrict__ sums) {
   __shared__ double scratch[kSpanBlock / WAVE_SIZE];
   typedef float V __attribute__((ext_vector_type(4), aligned(4)));
-  const int c = blockIdx.x;
+  const int c = mirrored_chunk();
+  if (c >= table.first[table.count]) return;
   const int s = span_of_chunk(table.first, table.count, c);
   const int chunk0 = table.first[s], chunk1 = table.first[s + 1];
   const uint32_t begin = uint32_t(c - chunk0) * table.chunk;
@@ -125,19 +127,22 @@ __global__ __launch_bounds__(kSpanBlock) void lamb_update_kernel(
     pp += d.x;
     uu += d.y;
   }
-  pp = block_sum_f64(pp, scratch);
-  uu = block_sum_f64(uu, scratch);
+  pp = block_sum_f64<kSpanBlock>(pp, scratch);
+  uu = block_sum_f64<kSpanBlock>(uu, scratch);
   const double ratio = (pp > 0.0 && uu > 0.0) ? sqrt(pp) / sqrt(uu) : 1.0;
   const float step = -static_cast<float>(r.lr * ratio);
   const uint32_t nv = n / 4;
   for (uint32_t i = threadIdx.x; i < nv; i += kSpanBlock) {
-    V pv = reinterpret_cast<const V*>(p)[i];
-    const V mv = reinterpret_cast<const V*>(m)[i];
-    const V vv = reinterpret_cast<const V*>(v)[i];
+    V* at = reinterpret_cast<V*>(p) + i;
+    V pv = __builtin_nontemporal_load(at);
+    const V mv =
+        __builtin_nontemporal_load(reinterpret_cast<const V*>(m) + i);
+    const V vv =
+        __builtin_nontemporal_load(reinterpret_cast<const V*>(v) + i);
     #pragma unroll
     for (int j = 0; j < 4; ++j)
       pv[j] = fmaf(step, lamb_rate(pv[j], mv[j], vv[j], decay, r), pv[j]);
-    reinterpret_cast<V*>(p)[i] = pv;
+    __builtin_nontemporal_store(pv, at);
   }
   const uint32_t t = nv * 4 + threadIdx.x;
   if (t < n) p[t] = fmaf(step, lamb_rate(p[t], m[t], v[t], decay, r), p[t]);
@@ -195,7 +200,7 @@ void launch_lamb_step(const std::vector<LambTensor>& tensors, SpanType type,
       hipLaunchKernelGGL((lamb_moments_kernel<decltype(value)>), grid, block,
                          0, stream, table, r, norm, max_norm, sums);
     });
-    hipLaunchKernelGGL(lamb_update_kernel, grid, block, 0, stream, table, r,
-                       sums);
+    hipLaunchKernelGGL(lamb_update_kernel, dim3((grid.x + 7) / 8 * 8), block,
+                       0, stream, table, r, sums);
   }
 }

@@ -30,7 +30,6 @@ void with_element_type(SpanType type, F f) {
     f(_Float16());
 }
 
-constexpr int kMaxSpans = 224;
 constexpr int kSpanBlock = 256;
 struct SpanTable {
   void* ptr[kMaxSpans];
@@ -64,7 +63,16 @@ __device__ __forceinline__ int span_of_chunk(const int* first, int count,
   return __builtin_amdgcn_readfirstlane(below - 1);
 }
 
-// Block sum in 64 bits, for blocks of kSpanBlock threads; valid in all threads.
+// The chunk of a second pass's block, which takes the chunks in the opposite
+// order of the first: it begins with what was read last, and each chunk is on
+// the XCD (blocks go to the 8 of them in turn) whose L2 has read it.  The grid
+// is a multiple of 8; a chunk past the last one is none.
+__device__ __forceinline__ int mirrored_chunk() {
+  return int(gridDim.x) - 8 - int(blockIdx.x & ~7u) + int(blockIdx.x & 7u);
+}
+
+// Block sum in 64 bits, for blocks of kThreads; valid in all threads.
+template <int kThreads>
 __device__ __forceinline__ double block_sum_f64(double v, double* scratch) {
   #pragma unroll
   for (int off = WAVE_SIZE / 2; off > 0; off >>= 1)
@@ -74,7 +82,7 @@ __device__ __forceinline__ double block_sum_f64(double v, double* scratch) {
   __syncthreads();
   double out = scratch[0];
   #pragma unroll
-  for (int w = 1; w < kSpanBlock / WAVE_SIZE; ++w) out += scratch[w];
+  for (int w = 1; w < kThreads / WAVE_SIZE; ++w) out += scratch[w];
   __syncthreads();
   return out;
 }

@@ -17,13 +17,16 @@
 
 int64_t grad_norm_partials(const std::vector<TensorSpan>& spans,
                            SpanType type);
-void launch_grad_norm_partial(const std::vector<TensorSpan>& spans,
-                              SpanType type, bool inf, double* partial,
-                              hipStream_t stream);
+int64_t launch_grad_norm_partial(const std::vector<TensorSpan>& spans,
+                                 SpanType type, bool inf, double* partial,
+                                 hipStream_t stream);
 void launch_grad_norm_finish(const double* partial, int64_t n, bool inf,
-                             double bound, float* out, hipStream_t stream);
+                             float* norm, hipStream_t stream);
+void launch_grad_norm_join(const double* partial, int64_t n, bool inf,
+                           double* joined, hipStream_t stream);
 void launch_grad_scale(const std::vector<TensorSpan>& spans, SpanType type,
-                       const float* factor, hipStream_t stream);
+                       bool inf, const double* partial, int64_t n,
+                       double bound, float* norm, hipStream_t stream);
 void launch_grad_clamp(const std::vector<TensorSpan>& spans, SpanType type,
                        float bound, hipStream_t stream);
 int64_t lamb_workspace_doubles();
@@ -34,99 +37,178 @@ void launch_lamb_step(const std::vector<LambTensor>& tensors, SpanType type,
 
 namespace {
 
-using Tensors = std::vector<torch::Tensor>;
 using Range = std::pair<uintptr_t, uintptr_t>;
 
-SpanType span_type(const torch::Tensor& t) {
+// A Python list of tensors, borrowed: the caller's list keeps them alive.
+class TensorList {
+ public:
+  TensorList(const pybind11::list& list, const char* what) {
+    PyObject* items = list.ptr();
+    const Py_ssize_t n = PyList_GET_SIZE(items);
+    refs_.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* item = PyList_GET_ITEM(items, i);
+      TORCH_CHECK_TYPE(THPVariable_Check(item), what,
+                       ": expected tensors, got ", Py_TYPE(item)->tp_name);
+      refs_.push_back(&THPVariable_Unpack(item));
+    }
+  }
+  size_t size() const { return refs_.size(); }
+  bool empty() const { return refs_.empty(); }
+  const torch::Tensor& operator[](size_t i) const { return *refs_[i]; }
+
+ private:
+  std::vector<const torch::Tensor*> refs_;
+};
+
+SpanType span_type(const torch::Tensor& t, const char* what) {
+  TORCH_CHECK_TYPE(t.layout() == at::kStrided, what,
+                   ": expected dense (strided) tensors");
   switch (t.scalar_type()) {
     case at::kFloat: return SpanType::kF32;
     case at::kBFloat16: return SpanType::kBF16;
     case at::kHalf: return SpanType::kF16;
     default:
-      TORCH_CHECK_TYPE(false, "expected fp32, bf16 or fp16 tensors, got ",
+      TORCH_CHECK_TYPE(false, what,
+                       ": expected fp32, bf16 or fp16 tensors, got ",
                        t.scalar_type());
   }
 }
 
-// What every list has to be; the same device comes last, so that the other
-// refusals are the same with and without a GPU.
-void check_list(const Tensors& list, const char* what) {
-  for (const auto& t : list) {
-    TORCH_CHECK_TYPE(t.defined() && t.layout() == at::kStrided, what,
-                     ": expected dense (strided) tensors");
-    span_type(t);
-  }
-}
-
-void check_device(const Tensors& list, const char* what,
+// Checked after everything else, so that the other refusals are the same with
+// and without a GPU.
+void check_device(const TensorList& list, const char* what,
                   const torch::Device& device) {
-  for (const auto& t : list)
-    TORCH_CHECK_VALUE(t.device() == device, what, ": expected all tensors on ",
-                      device, ", got one on ", t.device());
+  for (size_t i = 0; i < list.size(); ++i)
+    TORCH_CHECK_VALUE(list[i].device() == device, what,
+                      ": expected all tensors on ", device, ", got one on ",
+                      list[i].device());
   TORCH_CHECK_VALUE(device.is_cuda(), what, ": expected GPU tensors");
 }
 
-void add_range(std::vector<Range>& ranges, const torch::Tensor& t) {
-  if (t.numel() == 0) return;
-  // the addresses that a strided tensor reaches, strides being >= 0
-  int64_t reach = 1;
-  for (int64_t d = 0; d < t.dim(); ++d) reach += (t.size(d) - 1) * t.stride(d);
-  const auto begin = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-  ranges.emplace_back(begin, begin + reach * t.element_size());
-}
+// The memory that tensors reach, to see whether any two share some.
+class Ranges {
+ public:
+  explicit Ranges(size_t n) { ranges_.reserve(n); }
 
-void check_disjoint(std::vector<Range>& ranges, const char* what) {
-  if (!std::is_sorted(ranges.begin(), ranges.end()))
-    std::sort(ranges.begin(), ranges.end());
-  for (size_t i = 1; i < ranges.size(); ++i)
-    TORCH_CHECK_VALUE(ranges[i - 1].second <= ranges[i].first, what,
-                      ": a tensor is listed twice, or two share memory");
-}
+  static Range of(const torch::Tensor& t) {
+    int64_t reach = 1;  // in elements, strides being >= 0
+    if (t.is_non_overlapping_and_dense()) {
+      reach = t.numel();
+    } else {
+      for (int64_t d = 0; d < t.dim(); ++d)
+        reach += (t.size(d) - 1) * t.stride(d);
+    }
+    const auto begin = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    return {begin, begin + reach * t.element_size()};
+  }
 
-// `t` is only read, but from none of the (sorted, disjoint) ranges.
-void check_apart(const std::vector<Range>& ranges, const torch::Tensor& t,
-                 const char* what) {
-  std::vector<Range> own;
-  add_range(own, t);
-  if (own.empty() || ranges.empty()) return;
-  auto it = std::lower_bound(ranges.begin(), ranges.end(),
-                             Range(own[0].second, 0));
-  TORCH_CHECK_VALUE(
-      it == ranges.begin() || (it - 1)->second <= own[0].first, what,
-      ": a gradient shares memory with a parameter or a moment");
-}
+  void add(const torch::Tensor& t) {
+    if (t.numel() == 0) return;
+    const Range r = of(t);
+    ordered_ = ordered_ && (ranges_.empty() || ranges_.back() < r);
+    ranges_.push_back(r);
+  }
+
+  void check_disjoint(const char* what) {
+    if (!ordered_) std::sort(ranges_.begin(), ranges_.end());
+    for (size_t i = 1; i < ranges_.size(); ++i)
+      TORCH_CHECK_VALUE(ranges_[i - 1].second <= ranges_[i].first, what,
+                        ": a tensor is listed twice, or two share memory");
+  }
+
+  // Whether none of the (disjoint) ranges reaches into `t`'s.
+  bool apart_from(const torch::Tensor& t) const {
+    if (t.numel() == 0) return true;
+    const Range r = of(t);
+    const auto it =
+        std::lower_bound(ranges_.begin(), ranges_.end(), Range(r.second, 0));
+    return it == ranges_.begin() || (it - 1)->second <= r.first;
+  }
+
+ private:
+  std::vector<Range> ranges_;
+  bool ordered_ = true;
+};
 
 // Whether two tensors of one shape lay their elements out alike; the stride of
 // a dimension of length one says nothing.
 bool same_layout(const torch::Tensor& a, const torch::Tensor& b) {
+  if (a.strides() == b.strides()) return true;
   for (int64_t d = 0; d < a.dim(); ++d)
     if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
   return true;
 }
 
-// A list as spans.  Neighbours in memory that are neighbours in the list are
-// one span: the flat gradient buffer's views are a single one.
-struct Spans {
-  SpanType type;
-  std::vector<TensorSpan> spans;
-};
+// The kernels write through raw pointers: tell autograd, as an in-place
+// operation does.
+void mark_written(const TensorList& list) {
+  for (size_t i = 0; i < list.size(); ++i)
+    if (!list[i].is_inference()) list[i].unsafeGetTensorImpl()->bump_version();
+}
 
-std::vector<Spans> spans_by_type(const Tensors& list) {
-  std::vector<Spans> out;
-  for (const auto& t : list) {
-    int64_t left = t.numel();
-    if (left == 0) continue;
-    const SpanType type = span_type(t);
-    auto it = std::find_if(out.begin(), out.end(),
-                           [&](const Spans& s) { return s.type == type; });
-    if (it == out.end()) {
-      out.push_back({type, {}});
-      it = out.end() - 1;
+// A checked list of gradients as spans of memory, by type.  Neighbours in
+// memory that are neighbours in the list are one span: the flat gradient
+// buffer's views are a single one.  Tensors whose elements do not fill one
+// range of memory are worked on in a dense copy.
+class Gradients {
+ public:
+  Gradients(const TensorList& list, const char* what, bool write)
+      : device_(list[0].device()) {
+    const size_t n = list.size();
+    Ranges ranges(write ? n : 0);
+    std::vector<SpanType> types(n);
+    for (size_t i = 0; i < n; ++i) {
+      types[i] = span_type(list[i], what);
+      if (!write) continue;
+      TORCH_CHECK_VALUE(
+          list[i].is_non_overlapping_and_dense() ||
+              at::has_internal_overlap(list[i]) != at::MemOverlap::Yes,
+          what, ": elements of a tensor share memory (an expanded view); it "
+          "cannot be written in place");
+      ranges.add(list[i]);
     }
+    if (write) ranges.check_disjoint(what);
+    check_device(list, what, device_);
+    const c10::DeviceGuard guard(device_);
+    for (size_t i = 0; i < n; ++i) {
+      const auto& t = list[i];
+      if (t.numel() == 0) continue;
+      if (t.is_non_overlapping_and_dense()) {
+        add(t, types[i]);
+      } else {
+        copies_.emplace_back(&t, t.detach().contiguous());
+        add(copies_.back().second, types[i]);
+      }
+    }
+  }
+
+  struct Group {
+    SpanType type;
+    std::vector<TensorSpan> spans;
+  };
+  const std::vector<Group>& groups() const { return groups_; }
+  const torch::Device& device() const { return device_; }
+
+  void write_copies_back() const {
+    for (const auto& pair : copies_) pair.first->detach().copy_(pair.second);
+  }
+
+ private:
+  void add(const torch::Tensor& t, SpanType type) {
+    Group* group = nullptr;
+    for (Group& g : groups_)
+      if (g.type == type) group = &g;
+    if (group == nullptr) {
+      groups_.push_back({type, {}});
+      group = &groups_.back();
+    }
+    auto& spans = group->spans;
+    int64_t left = t.numel();
     const int64_t size = t.element_size();
     auto* ptr = static_cast<char*>(const_cast<void*>(t.const_data_ptr()));
-    if (!it->spans.empty()) {
-      TensorSpan& last = it->spans.back();
+    if (!spans.empty()) {
+      TensorSpan& last = spans.back();
       if (static_cast<char*>(last.ptr) + last.len * size == ptr) {
         const int64_t more = std::min(left, kMaxSpanLen - last.len);
         last.len += more;
@@ -136,161 +218,147 @@ std::vector<Spans> spans_by_type(const Tensors& list) {
     }
     while (left > 0) {
       const int64_t n = std::min(left, kMaxSpanLen);
-      it->spans.push_back({ptr, n});
+      spans.push_back({ptr, n});
       ptr += n * size;
       left -= n;
     }
   }
-  return out;
-}
 
-// Tensors whose elements do not fill one range of memory are worked on in a
-// dense copy; `back` holds (tensor, copy) to be written back.
-Tensors dense_list(const Tensors& list,
-                   std::vector<std::pair<torch::Tensor, torch::Tensor>>* back) {
-  Tensors out;
-  out.reserve(list.size());
-  for (const auto& t : list) {
-    if (t.is_non_overlapping_and_dense()) {
-      out.push_back(t);
-    } else {
-      out.push_back(t.contiguous());
-      if (back != nullptr) back->emplace_back(t, out.back());
-    }
-  }
-  return out;
-}
+  torch::Device device_;
+  std::vector<Group> groups_;
+  std::vector<std::pair<const torch::Tensor*, torch::Tensor>> copies_;
+};
 
-// The kernels write through raw pointers: tell autograd, as an in-place
-// operation does.
-void mark_written(const Tensors& list) {
-  for (const auto& t : list)
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-
-void check_writable(const Tensors& list, const char* what) {
-  std::vector<Range> ranges;
-  ranges.reserve(list.size());
-  for (const auto& t : list) {
-    TORCH_CHECK_VALUE(
-        at::has_internal_overlap(t) != at::MemOverlap::Yes, what,
-        ": elements of a tensor share memory (an expanded view); it cannot "
-        "be written in place");
-    add_range(ranges, t);
-  }
-  check_disjoint(ranges, what);
-}
-
-// [norm, factor] of a non-empty list
-torch::Tensor norm_and_factor(const Tensors& dense, bool inf, double bound) {
-  const auto stream = at::hip::getCurrentHIPStream();
-  const auto groups = spans_by_type(dense);
+// The partial results of a list's norm.
+torch::Tensor norm_partials(const Gradients& grads, bool inf,
+                            hipStream_t stream) {
   int64_t n = 0;
-  for (const auto& g : groups) n += grad_norm_partials(g.spans, g.type);
-  const auto options = dense[0].options().requires_grad(false);
-  auto partial = torch::empty({n}, options.dtype(at::kDouble));
-  auto out = torch::empty({2}, options.dtype(at::kFloat));
+  for (const auto& g : grads.groups()) n += grad_norm_partials(g.spans, g.type);
+  auto partial = torch::empty(
+      {n}, torch::TensorOptions().dtype(at::kDouble).device(grads.device()));
   double* at = partial.data_ptr<double>();
-  for (const auto& g : groups) {
-    launch_grad_norm_partial(g.spans, g.type, inf, at, stream);
-    at += grad_norm_partials(g.spans, g.type);
-  }
-  launch_grad_norm_finish(partial.data_ptr<double>(), n, inf, bound,
-                          out.data_ptr<float>(), stream);
-  C10_HIP_CHECK(hipGetLastError());
-  return out;
+  for (const auto& g : grads.groups())
+    at += launch_grad_norm_partial(g.spans, g.type, inf, at, stream);
+  return partial;
 }
 
-torch::Tensor grad_norm(const Tensors& grads, bool inf) {
+torch::Tensor one_float(const torch::Device& device) {
+  return torch::empty({},
+                      torch::TensorOptions().dtype(at::kFloat).device(device));
+}
+
+torch::Tensor grad_norm(const pybind11::list& list, bool inf) {
   const char* what = "global_grad_norm";
-  TORCH_CHECK_VALUE(!grads.empty(), what, ": no tensors");
-  check_list(grads, what);
-  check_device(grads, what, grads[0].device());
-  const c10::DeviceGuard guard(grads[0].device());
-  const auto dense = dense_list(grads, nullptr);
-  return norm_and_factor(dense, inf, 0.0).select(0, 0);
+  const TensorList tensors(list, what);
+  TORCH_CHECK_VALUE(!tensors.empty(), what, ": no tensors");
+  const Gradients grads(tensors, what, false);
+  const c10::DeviceGuard guard(grads.device());
+  const auto stream = at::hip::getCurrentHIPStream();
+  const auto partial = norm_partials(grads, inf, stream);
+  auto norm = one_float(grads.device());
+  launch_grad_norm_finish(partial.data_ptr<double>(), partial.numel(), inf,
+                          norm.data_ptr<float>(), stream);
+  C10_HIP_CHECK(hipGetLastError());
+  return norm;
 }
 
-torch::Tensor grad_clip_norm(const Tensors& grads, double max_norm, bool inf) {
+torch::Tensor grad_clip_norm(const pybind11::list& list, double max_norm,
+                             bool inf) {
   const char* what = "clip_grads_by_norm_";
-  TORCH_CHECK_VALUE(!grads.empty(), what, ": no tensors");
+  const TensorList tensors(list, what);
+  TORCH_CHECK_VALUE(!tensors.empty(), what, ": no tensors");
   TORCH_CHECK_VALUE(max_norm >= 0.0, what, ": max_norm must be >= 0, got ",
                     max_norm);
-  check_list(grads, what);
-  check_writable(grads, what);
-  check_device(grads, what, grads[0].device());
-  const c10::DeviceGuard guard(grads[0].device());
-  std::vector<std::pair<torch::Tensor, torch::Tensor>> back;
-  const auto dense = dense_list(grads, &back);
-  auto out = norm_and_factor(dense, inf, max_norm);
+  const Gradients grads(tensors, what, true);
+  const c10::DeviceGuard guard(grads.device());
   const auto stream = at::hip::getCurrentHIPStream();
-  for (const auto& g : spans_by_type(dense))
-    launch_grad_scale(g.spans, g.type, out.data_ptr<float>() + 1, stream);
+  auto partial = norm_partials(grads, inf, stream);
+  const double* sums = partial.data_ptr<double>();
+  int64_t n = partial.numel();
+  auto norm = one_float(grads.device());
+  torch::Tensor joined;
+  if (n > kMaxJoinedPartials || n == 0) {
+    // too many for every block of the scaling pass to join them: it gets one
+    joined = torch::empty({1}, partial.options());
+    launch_grad_norm_join(sums, n, inf, joined.data_ptr<double>(), stream);
+    sums = joined.data_ptr<double>();
+    n = 1;
+  }
+  float* out = norm.data_ptr<float>();
+  if (grads.groups().empty())
+    launch_grad_norm_finish(sums, n, inf, out, stream);
+  for (const auto& g : grads.groups()) {
+    launch_grad_scale(g.spans, g.type, inf, sums, n, max_norm, out, stream);
+    out = nullptr;  // the first launch writes the norm
+  }
   C10_HIP_CHECK(hipGetLastError());
-  for (auto& pair : back) pair.first.detach().copy_(pair.second);
-  mark_written(grads);
-  return out.select(0, 0);
+  grads.write_copies_back();
+  mark_written(tensors);
+  return norm;
 }
 
-void grad_clip_value(const Tensors& grads, double clip_value) {
+void grad_clip_value(const pybind11::list& list, double clip_value) {
   const char* what = "clip_grads_by_value_";
+  const TensorList tensors(list, what);
   TORCH_CHECK_VALUE(clip_value >= 0.0, what,
                     ": clip_value must be >= 0, got ", clip_value);
-  if (grads.empty()) return;
-  check_list(grads, what);
-  check_writable(grads, what);
-  check_device(grads, what, grads[0].device());
-  const c10::DeviceGuard guard(grads[0].device());
-  std::vector<std::pair<torch::Tensor, torch::Tensor>> back;
-  const auto dense = dense_list(grads, &back);
+  if (tensors.empty()) return;
+  const Gradients grads(tensors, what, true);
+  const c10::DeviceGuard guard(grads.device());
   const auto stream = at::hip::getCurrentHIPStream();
-  for (const auto& g : spans_by_type(dense))
+  for (const auto& g : grads.groups())
     launch_grad_clamp(g.spans, g.type, static_cast<float>(clip_value), stream);
   C10_HIP_CHECK(hipGetLastError());
-  for (auto& pair : back) pair.first.detach().copy_(pair.second);
-  mark_written(grads);
+  grads.write_copies_back();
+  mark_written(tensors);
 }
 
-void lamb_step(const Tensors& params, const Tensors& grads,
-               const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
+void lamb_step(const pybind11::list& param_list,
+               const pybind11::list& grad_list,
+               const pybind11::list& exp_avg_list,
+               const pybind11::list& exp_avg_sq_list,
                const std::vector<double>& decay, int64_t step, double lr,
                double beta1, double beta2, double eps, double max_norm,
                const c10::optional<torch::Tensor>& norm) {
   const char* what = "fused_lamb_step";
+  const TensorList params(param_list, what), grads(grad_list, what),
+      exp_avgs(exp_avg_list, what), exp_avg_sqs(exp_avg_sq_list, what);
   const size_t n = params.size();
   TORCH_CHECK_VALUE(grads.size() == n && exp_avgs.size() == n &&
                         exp_avg_sqs.size() == n && decay.size() == n,
                     what, ": lists of different lengths");
   TORCH_CHECK_VALUE(step >= 1, what, ": step counts from 1, got ", step);
   if (n == 0) return;
-  std::vector<Range> ranges;
-  ranges.reserve(4 * n);
+  Ranges written(3 * n);
   for (const auto* list : {&params, &exp_avgs, &exp_avg_sqs}) {
-    check_list(*list, what);
     for (size_t i = 0; i < n; ++i) {
       const auto& t = (*list)[i];
-      TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, what,
+      const auto& p = params[i];
+      TORCH_CHECK_TYPE(span_type(t, what) == SpanType::kF32, what,
                        ": parameters and moments must be fp32, got ",
                        t.scalar_type());
       TORCH_CHECK_VALUE(t.is_non_overlapping_and_dense(), what,
                         ": parameters and moments must be dense");
       TORCH_CHECK_VALUE(t.numel() < (int64_t(1) << 31), what,
                         ": a parameter has 2^31 elements or more");
-      TORCH_CHECK_VALUE(
-          t.sizes() == params[i].sizes() && same_layout(t, params[i]),
-          what, ": moments must have their parameter's shape and strides");
-      add_range(ranges, t);
+      TORCH_CHECK_VALUE(t.sizes() == p.sizes() && same_layout(t, p), what,
+                        ": moments must have their parameter's shape and "
+                        "strides");
+      written.add(t);
     }
   }
-  check_list(grads, what);
+  const SpanType grad_type = span_type(grads[0], what);
   for (size_t i = 0; i < n; ++i) {
+    TORCH_CHECK_TYPE(span_type(grads[i], what) == grad_type, what,
+                     ": gradients of different types");
     TORCH_CHECK_VALUE(grads[i].sizes() == params[i].sizes(), what,
                       ": a gradient has another shape than its parameter");
-    TORCH_CHECK_TYPE(grads[i].scalar_type() == grads[0].scalar_type(), what,
-                     ": gradients of different types");
   }
-  check_disjoint(ranges, what);
-  for (const auto& g : grads) check_apart(ranges, g, what);
+  written.check_disjoint(what);
+  for (size_t i = 0; i < n; ++i)
+    TORCH_CHECK_VALUE(written.apart_from(grads[i]), what,
+                      ": a gradient shares memory with a parameter or a "
+                      "moment");
   const auto device = params[0].device();
   for (const auto* list : {&params, &grads, &exp_avgs, &exp_avg_sqs})
     check_device(*list, what, device);
@@ -303,30 +371,29 @@ void lamb_step(const Tensors& params, const Tensors& grads,
     norm_ptr = norm->data_ptr<float>();
   }
   const c10::DeviceGuard guard(device);
-  Tensors held;  // gradients in the parameters' layout, until the launches
+  std::vector<torch::Tensor> held;  // gradients in their parameters' layout
   std::vector<LambTensor> list;
   list.reserve(n);
   for (size_t i = 0; i < n; ++i) {
     const auto& p = params[i];
     if (p.numel() == 0) continue;
-    torch::Tensor g = grads[i];
-    if (!same_layout(g, p)) {
-      g = torch::empty_strided(p.sizes(), p.strides(), g.options()
-                                   .requires_grad(false))
-              .copy_(g.detach());
-      held.push_back(g);
+    const void* g = grads[i].const_data_ptr();
+    if (!same_layout(grads[i], p)) {
+      held.push_back(torch::empty_strided(
+          p.sizes(), p.strides(), grads[i].options().requires_grad(false)));
+      held.back().copy_(grads[i].detach());
+      g = held.back().const_data_ptr();
     }
-    list.push_back({p.data_ptr<float>(), g.const_data_ptr(),
-                    exp_avgs[i].data_ptr<float>(),
+    list.push_back({p.data_ptr<float>(), g, exp_avgs[i].data_ptr<float>(),
                     exp_avg_sqs[i].data_ptr<float>(), p.numel(),
                     static_cast<float>(decay[i])});
   }
   if (list.empty()) return;
   auto workspace = torch::empty(
       {lamb_workspace_doubles()},
-      params[0].options().dtype(at::kDouble).requires_grad(false));
-  launch_lamb_step(list, span_type(grads[0]), lr, beta1, beta2, eps, step,
-                   norm_ptr, max_norm, workspace.data_ptr<double>(),
+      torch::TensorOptions().dtype(at::kDouble).device(device));
+  launch_lamb_step(list, grad_type, lr, beta1, beta2, eps, step, norm_ptr,
+                   max_norm, workspace.data_ptr<double>(),
                    at::hip::getCurrentHIPStream());
   C10_HIP_CHECK(hipGetLastError());
   mark_written(params);

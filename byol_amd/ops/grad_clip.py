@@ -40,7 +40,7 @@ def _is_inf(norm_type: float) -> bool:
 def _on_gpu(grads: Sequence[torch.Tensor], what: str) -> bool:
     """Whether the HIP kernels take the list (their binding then checks it);
     a list on the CPU is checked here."""
-    if any(t.is_cuda for t in grads):
+    if grads[0].is_cuda or any(t.is_cuda for t in grads):
         return True
     for t in grads:
         if t.dtype not in _DTYPES or t.layout is not torch.strided:
@@ -75,7 +75,6 @@ def _reference_norm(grads, inf: bool) -> torch.Tensor:
     return torch.stack(parts).sum().sqrt()
 
 
-@torch.no_grad()
 def global_grad_norm(grads: Sequence[torch.Tensor],
                      norm_type: float = 2.0) -> torch.Tensor:
     """The 2-norm (or, with ``math.inf``, the largest magnitude) of all
@@ -87,10 +86,10 @@ def global_grad_norm(grads: Sequence[torch.Tensor],
         return torch.zeros(())
     if _on_gpu(grads, "global_grad_norm"):
         return require_extension("global_grad_norm").grad_norm(grads, inf)
-    return _reference_norm(grads, inf).float()
+    with torch.no_grad():
+        return _reference_norm(grads, inf).float()
 
 
-@torch.no_grad()
 def clip_grads_by_norm_(grads: Sequence[torch.Tensor], max_norm: float,
                         norm_type: float = 2.0) -> torch.Tensor:
     """Scale all tensors in place by ``min(1, max_norm / (norm + 1e-6))``,
@@ -107,15 +106,15 @@ def clip_grads_by_norm_(grads: Sequence[torch.Tensor], max_norm: float,
     if _on_gpu(grads, what):
         return require_extension(what).grad_clip_norm(grads, max_norm, inf)
     _check_writable(grads, what)
-    norm = _reference_norm(grads, inf)
-    factor = (max_norm / (norm + 1e-6)).clamp(max=1.0).float()
-    if factor != 1.0:
-        for t in grads:
-            t.copy_(t.float() * factor)
-    return norm.float()
+    with torch.no_grad():
+        norm = _reference_norm(grads, inf)
+        factor = (max_norm / (norm + 1e-6)).clamp(max=1.0).float()
+        if factor != 1.0:
+            for t in grads:
+                t.copy_(t.float() * factor)
+        return norm.float()
 
 
-@torch.no_grad()
 def clip_grads_by_value_(grads: Sequence[torch.Tensor],
                          clip_value: float) -> None:
     """Bound every element to ``[-clip_value, clip_value]`` in place; NaN
@@ -131,5 +130,6 @@ def clip_grads_by_value_(grads: Sequence[torch.Tensor],
         require_extension(what).grad_clip_value(grads, clip_value)
         return
     _check_writable(grads, what)
-    for t in grads:
-        t.copy_(t.float().clamp(-clip_value, clip_value))
+    with torch.no_grad():
+        for t in grads:
+            t.copy_(t.float().clamp(-clip_value, clip_value))
