@@ -29,11 +29,13 @@ void launch_grad_scale(const std::vector<TensorSpan>& spans, SpanType type,
                        double bound, float* norm, hipStream_t stream);
 void launch_grad_clamp(const std::vector<TensorSpan>& spans, SpanType type,
                        float bound, hipStream_t stream);
-int64_t lamb_workspace_doubles();
-void launch_lamb_step(const std::vector<LambTensor>& tensors, SpanType type,
-                      double lr, double beta1, double beta2, double eps,
-                      int64_t step, const float* norm, double max_norm,
-                      double* workspace, hipStream_t stream);
+int64_t lamb_chunks(const std::vector<LambTensor>& tensors);
+int64_t lamb_workspace_bytes(int64_t count, int64_t chunks);
+void launch_lamb_step(std::vector<LambTensor>& tensors, int64_t chunks,
+                      SpanType type, double lr, double beta1, double beta2,
+                      double eps, int64_t step, const float* norm,
+                      double max_norm, int64_t wait_ticks, void* workspace,
+                      hipStream_t stream);
 
 namespace {
 
@@ -319,7 +321,7 @@ void lamb_step(const pybind11::list& param_list,
                const pybind11::list& exp_avg_sq_list,
                const std::vector<double>& decay, int64_t step, double lr,
                double beta1, double beta2, double eps, double max_norm,
-               const c10::optional<torch::Tensor>& norm) {
+               const c10::optional<torch::Tensor>& norm, int64_t wait_ticks) {
   const char* what = "fused_lamb_step";
   const TensorList params(param_list, what), grads(grad_list, what),
       exp_avgs(exp_avg_list, what), exp_avg_sqs(exp_avg_sq_list, what);
@@ -328,6 +330,8 @@ void lamb_step(const pybind11::list& param_list,
                         exp_avg_sqs.size() == n && decay.size() == n,
                     what, ": lists of different lengths");
   TORCH_CHECK_VALUE(step >= 1, what, ": step counts from 1, got ", step);
+  TORCH_CHECK_VALUE(wait_ticks >= 0 && wait_ticks <= 100000, what,
+                    ": wait_ticks must be 0 to 100000, got ", wait_ticks);
   if (n == 0) return;
   Ranges written(3 * n);
   for (const auto* list : {&params, &exp_avgs, &exp_avg_sqs}) {
@@ -389,11 +393,13 @@ void lamb_step(const pybind11::list& param_list,
                     static_cast<float>(decay[i])});
   }
   if (list.empty()) return;
+  const int64_t chunks = lamb_chunks(list);
+  TORCH_CHECK_VALUE(chunks < (int64_t(1) << 30), what, ": too many elements");
   auto workspace = torch::empty(
-      {lamb_workspace_doubles()},
-      torch::TensorOptions().dtype(at::kDouble).device(device));
-  launch_lamb_step(list, grad_type, lr, beta1, beta2, eps, step, norm_ptr,
-                   max_norm, workspace.data_ptr<double>(),
+      {lamb_workspace_bytes(static_cast<int64_t>(list.size()), chunks)},
+      torch::TensorOptions().dtype(at::kByte).device(device));
+  launch_lamb_step(list, chunks, grad_type, lr, beta1, beta2, eps, step,
+                   norm_ptr, max_norm, wait_ticks, workspace.data_ptr(),
                    at::hip::getCurrentHIPStream());
   C10_HIP_CHECK(hipGetLastError());
   mark_written(params);
@@ -415,5 +421,8 @@ void bind_optim(pybind11::module& mod) {
           pybind11::arg("decay"), pybind11::arg("step"), pybind11::arg("lr"),
           pybind11::arg("beta1"), pybind11::arg("beta2"),
           pybind11::arg("eps"), pybind11::arg("max_norm"),
-          pybind11::arg("norm") = pybind11::none());
+          pybind11::arg("norm") = pybind11::none(),
+          // how long a block waits for the others of its tensor, in 10 ns
+          // units; without a wait all long tensors take the second pass
+          pybind11::arg("wait_ticks") = 20000);
 }

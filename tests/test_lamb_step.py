@@ -128,7 +128,8 @@ def test_step(device, dtype, step, clip, sizes):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("sizes", [[5_000_001, 3, 700_000],
-                                   [70_000] * 100])
+                                   [70_000] * 100,
+                                   [10_000_003, 8192, 8193, 9_000_000]])
 def test_large_lists(sizes):
     _, lists = make(sizes, "cuda", gap=1)
     before = [[t.clone() for t in ts] for ts in lists]
@@ -138,6 +139,23 @@ def test_large_lists(sizes):
     again = [[t.clone() for t in ts] for ts in before]
     ops.fused_lamb_step(*again, step=7, lr=0.01, weight_decay=decay)
     for a, b in zip(lists, again):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("wait_ticks", [0, 1, 1000])
+def test_second_pass_gives_the_same_bits(dtype, wait_ticks):
+    """Blocks that do not wait for the rest of their tensor, or give up, leave
+    it to a pass that computes the same."""
+    sizes = [3_000_001, 8192, 8193, 20_000, 5, 100_000] * 3
+    results = []
+    for ticks in (20000, wait_ticks):
+        _, lists = make(sizes, "cuda", dtype, gap=1)
+        ops.extension().lamb_step(*lists, [0.01] * len(sizes), 3, 0.1, B1, B2,
+                                  1e-6, 0.0, None, ticks)
+        results.append(lists)
+    for a, b in zip(*results):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
@@ -353,6 +371,30 @@ def test_two_streams():
     for lists, b in zip(made, before):
         norm = torch.cat([g.cpu().double() for g in b[1]]).norm().item()
         check(lists, b, 5, 0.1, 1e-6, [0.0, 0.0], 1.0 / (norm + 1e-6))
+
+
+@pytest.mark.gpu
+def test_two_large_steps_at_once():
+    """Steps that do not fit the chip together, on two streams: blocks that
+    wait for ones that cannot start give up, and the values are the same."""
+    sizes = [6_000_000, 70, 5_000_001, 300_000, 6_000_000]
+    decay = [0.01] * len(sizes)
+    made = [make(sizes, "cuda", seed=s)[1] for s in (1, 2, 1, 2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for step in range(1, 6):
+        for lists, s in zip(made, streams):
+            with torch.cuda.stream(s):
+                ops.fused_lamb_step(*lists, step=step, lr=0.1,
+                                    weight_decay=decay)
+    torch.cuda.synchronize()
+    for step in range(1, 6):
+        for lists in made[2:]:
+            ops.fused_lamb_step(*lists, step=step, lr=0.1, weight_decay=decay)
+    torch.cuda.synchronize()
+    for a, b in zip(made[:2], made[2:]):
+        for x, y in zip(a, b):
+            assert all(torch.equal(t, u) for t, u in zip(x, y))
 
 
 def engine_args(tmp_path, device, *extra):
