@@ -97,9 +97,78 @@ constexpr int kUnroll = 4;
 // The single block that joins all partial results.
 constexpr int kJoinBlock = 1024;
 
+// Joins partial results in a fixed order, for blocks of kThreads: load4(i, v)
+// gets those of i, i + kThreads, ... for a thread, load(i) one.  The sum of
+// squares or the largest magnitude, in all threads.
+template <typename Reduce, int kThreads, typename Load>
+__device__ __forceinline__ double join_partials(int n, double* scratch,
+                                                Load load) {
+  Reduce red;
+  int i = threadIdx.x;
+  for (; i + 3 * kThreads < n; i += 4 * kThreads) {
+    double v[4];
+    load(i, v, 4);
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) red.merge(v[k], k);
+  }
+  for (; i < n; i += kThreads) {
+    double v[1];
+    load(i, v, 1);
+    red.merge(v[0], 0);
+  }
+  return red.template join<kThreads>(scratch);
+}
+
+// From a launch that has ended.
+template <int kThreads>
+struct LoadPartials {
+  const double* partial;
+  __device__ __forceinline__ void operator()(int i, double* v, int n) const {
+    #pragma unroll
+    for (int k = 0; k < n; ++k) v[k] = partial[i + k * kThreads];
+  }
+};
+
+// From blocks that may still run: waits for each sum and takes it out.
+template <int kThreads>
+struct TakePartials {
+  uint64_t* sums;
+  uint64_t until;
+  __device__ __forceinline__ void operator()(int i, double* v, int n) const {
+    uint64_t bits[4];
+    #pragma unroll
+    for (int k = 0; k < n; ++k) bits[k] = load_sum(sums + i + k * kThreads);
+    #pragma unroll
+    for (int k = 0; k < n; ++k) {
+      uint64_t* at = sums + i + k * kThreads;
+      while (bits[k] == kNoSum && wall_clock64() < until) {
+        __builtin_amdgcn_s_sleep(1);
+        bits[k] = load_sum(at);
+      }
+      *at = kNoSum;
+      v[k] = sum_value(bits[k]);
+    }
+  }
+};
+
+// How the partial results become a norm.  With `sums`, the last block of the
+// call's last launch joins them as they come in: a launch less, 3 us for the
+// host and 4 us for the GPU.  It waits for blocks that wait for nothing
+// themselves and were started before it.  The time limit is for a device that
+// has failed; the norm is NaN then.
+struct NormEnd {
+  uint64_t* sums;  // kNoSum in all before and after the call; or null
+  int all;         // blocks of all launches of the call
+  double* joined;
+  float* norm;
+};
+
+constexpr uint64_t kJoinTicks = 1000000000;  // of 10 ns
+
 template <typename T, typename Reduce>
 __global__ __launch_bounds__(kSpanBlock) void grad_norm_partial_kernel(
-    const SpanTable table, double* __restrict__ partial) {
+    const SpanTable table, double* __restrict__ partial, int at,
+    const NormEnd end) {
   __shared__ double scratch[kSpanBlock / WAVE_SIZE];
   using V = typename Pack<T>::type;
   constexpr int L = Pack<T>::kLen;
@@ -123,22 +192,19 @@ __global__ __launch_bounds__(kSpanBlock) void grad_norm_partial_kernel(
   const uint32_t t = chunk.packs * L + threadIdx.x;
   if (t < chunk.n) red.add(static_cast<float>(chunk.data[t]), 0);
   const double sum = red.template join<kSpanBlock>(scratch);
-  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
-}
-
-// Joins partial results in a fixed order, for blocks of kThreads; the sum of
-// squares or the largest magnitude, in all threads.
-template <typename Reduce, int kThreads>
-__device__ __forceinline__ double join_partials(
-    const double* __restrict__ partial, int n, double* scratch) {
-  Reduce red;
-  int i = threadIdx.x;
-  for (; i + 3 * kThreads < n; i += 4 * kThreads) {
-    #pragma unroll
-    for (int k = 0; k < 4; ++k) red.merge(partial[i + k * kThreads], k);
+  const int own = at + blockIdx.x;
+  if (end.sums == nullptr) {
+    if (threadIdx.x == 0) partial[own] = sum;
+    return;
   }
-  for (; i < n; i += kThreads) red.merge(partial[i], 0);
-  return red.template join<kThreads>(scratch);
+  if (threadIdx.x == 0) store_sum(end.sums + own, sum);
+  if (own != end.all - 1) return;
+  const double all = join_partials<Reduce, kSpanBlock>(
+      end.all, scratch,
+      TakePartials<kSpanBlock>{end.sums, wall_clock64() + kJoinTicks});
+  if (threadIdx.x != 0) return;
+  *end.joined = all;
+  *end.norm = static_cast<float>(Reduce::norm(all));
 }
 
 // One block: the norm, or (for a scaling pass over many tables) one partial
@@ -148,7 +214,8 @@ __global__ __launch_bounds__(kJoinBlock) void grad_norm_finish_kernel(
     const double* __restrict__ partial, int n, float* __restrict__ norm,
     double* __restrict__ joined) {
   __shared__ double scratch[kJoinBlock / WAVE_SIZE];
-  const double all = join_partials<Reduce, kJoinBlock>(partial, n, scratch);
+  const double all = join_partials<Reduce, kJoinBlock>(
+      n, scratch, LoadPartials<kJoinBlock>{partial});
   if (threadIdx.x != 0) return;
   if (joined != nullptr)
     *joined = all;
@@ -198,7 +265,8 @@ __global__ __launch_bounds__(kSpanBlock) void grad_scale_kernel(
     double bound, float* __restrict__ norm_out) {
   __shared__ double scratch[kSpanBlock / WAVE_SIZE];
   const double norm =
-      Reduce::norm(join_partials<Reduce, kSpanBlock>(partial, n, scratch));
+      Reduce::norm(join_partials<Reduce, kSpanBlock>(
+          n, scratch, LoadPartials<kSpanBlock>{partial}));
   if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0)
     *norm_out = static_cast<float>(norm);
   const double ratio = bound / (norm + 1e-6);
@@ -256,13 +324,15 @@ int64_t for_tables(const std::vector<TensorSpan>& spans, SpanType type, F f) {
 
 template <typename Reduce>
 int64_t launch_partials(const std::vector<TensorSpan>& spans, SpanType type,
-                        double* partial, hipStream_t stream) {
+                        double* partial, int64_t at, const NormEnd& end,
+                        hipStream_t stream) {
   return for_tables(spans, type, [&](const SpanTable& t, int chunks,
                                      int64_t done) {
     with_element_type(type, [&](auto value) {
       hipLaunchKernelGGL(
           (grad_norm_partial_kernel<decltype(value), Reduce>), dim3(chunks),
-          dim3(kSpanBlock), 0, stream, t, partial + done);
+          dim3(kSpanBlock), 0, stream, t, partial,
+          static_cast<int>(at + done), end);
     });
   });
 }
@@ -301,9 +371,14 @@ int64_t grad_norm_partials(const std::vector<TensorSpan>& spans,
 
 int64_t launch_grad_norm_partial(const std::vector<TensorSpan>& spans,
                                  SpanType type, bool inf, double* partial,
+                                 int64_t at, int64_t all, uint64_t* sums,
+                                 double* joined, float* norm,
                                  hipStream_t stream) {
-  return inf ? launch_partials<LargestMagnitude>(spans, type, partial, stream)
-             : launch_partials<SumOfSquares>(spans, type, partial, stream);
+  const NormEnd end = {sums, static_cast<int>(all), joined, norm};
+  return inf ? launch_partials<LargestMagnitude>(spans, type, partial, at, end,
+                                                 stream)
+             : launch_partials<SumOfSquares>(spans, type, partial, at, end,
+                                             stream);
 }
 
 void launch_grad_norm_finish(const double* partial, int64_t n, bool inf,

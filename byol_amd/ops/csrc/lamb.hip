@@ -37,10 +37,6 @@ constexpr int kLdsPacks = 9;  // of them with p in LDS, the others in registers
 constexpr int kLambChunk = kLambBlock * 4 * kPacks;
 constexpr int kBlocksPerCu = 2;
 
-// A sum that is not there yet.  No sum has these bits: a NaN that comes from
-// 32-bit values has zeros at the end.
-constexpr uint64_t kNoSum = ~uint64_t(0);
-
 // The tensors of a step in device memory, and what its blocks tell each other.
 struct LambList {
   float** p;
@@ -122,15 +118,6 @@ __device__ __forceinline__ float lamb_factor(double pp, double uu, float lr) {
   return -static_cast<float>(lr * ratio);
 }
 
-__device__ __forceinline__ uint64_t load_sum(const uint64_t* at) {
-  return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-__device__ __forceinline__ void store_sum(uint64_t* at, double v) {
-  __hip_atomic_store(at, static_cast<uint64_t>(__double_as_longlong(v)),
-                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 // Adds up the sums of chunks [c0, c1) over the block, in a fixed order.  Each
 // sum is valid by itself (it is not kNoSum), so no other order between blocks
 // is needed.  With `wait`, sums that are missing are waited for until the time
@@ -153,8 +140,8 @@ __device__ __forceinline__ bool join_sums(const uint64_t* sums, int c0, int c1,
       a = load_sum(sums + 2 * k);
       b = load_sum(sums + 2 * k + 1);
     }
-    p += __longlong_as_double(static_cast<long long>(a));
-    u += __longlong_as_double(static_cast<long long>(b));
+    p += sum_value(a);
+    u += sum_value(b);
   }
   all = __syncthreads_and(all);
   *pp = block_sum_f64<kLambBlock>(p, scratch);

@@ -86,3 +86,25 @@ __device__ __forceinline__ double block_sum_f64(double v, double* scratch) {
   __syncthreads();
   return out;
 }
+
+// Sums that blocks tell each other while they run: 64 bits that are written
+// and read past the XCDs' own L2, and valid by themselves, so that no order
+// between other accesses is needed (a release or acquire at this scope writes
+// back or drops a whole L2: 1536 of them cost 70 us).
+//
+// A sum that is not there yet; no sum has these bits, as a NaN that comes from
+// 32-bit values has zeros at its end.
+constexpr uint64_t kNoSum = ~uint64_t(0);
+
+__device__ __forceinline__ uint64_t load_sum(const uint64_t* at) {
+  return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ void store_sum(uint64_t* at, double v) {
+  __hip_atomic_store(at, static_cast<uint64_t>(__double_as_longlong(v)),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ double sum_value(uint64_t bits) {
+  return __longlong_as_double(static_cast<long long>(bits));
+}

@@ -7,9 +7,12 @@
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
+#include <c10/hip/HIPFunctions.h>
 
 #include <algorithm>
 #include <cmath>
+#include <map>
+#include <mutex>
 #include <utility>
 #include <vector>
 
@@ -19,6 +22,8 @@ int64_t grad_norm_partials(const std::vector<TensorSpan>& spans,
                            SpanType type);
 int64_t launch_grad_norm_partial(const std::vector<TensorSpan>& spans,
                                  SpanType type, bool inf, double* partial,
+                                 int64_t at, int64_t all, uint64_t* sums,
+                                 double* joined, float* norm,
                                  hipStream_t stream);
 void launch_grad_norm_finish(const double* partial, int64_t n, bool inf,
                              float* norm, hipStream_t stream);
@@ -231,22 +236,62 @@ class Gradients {
   std::vector<std::pair<const torch::Tensor*, torch::Tensor>> copies_;
 };
 
-// The partial results of a list's norm.
-torch::Tensor norm_partials(const Gradients& grads, bool inf,
-                            hipStream_t stream) {
-  int64_t n = 0;
-  for (const auto& g : grads.groups()) n += grad_norm_partials(g.spans, g.type);
-  auto partial = torch::empty(
-      {n}, torch::TensorOptions().dtype(at::kDouble).device(grads.device()));
-  double* at = partial.data_ptr<double>();
-  for (const auto& g : grads.groups())
-    at += launch_grad_norm_partial(g.spans, g.type, inf, at, stream);
-  return partial;
-}
-
 torch::Tensor one_float(const torch::Device& device) {
   return torch::empty({},
                       torch::TensorOptions().dtype(at::kFloat).device(device));
+}
+
+// Places for the sums that a norm's blocks tell each other, "none" in all of
+// them between calls, for the current stream of the current device.  Calls on
+// one stream follow each other, so they share it; calls on other streams have
+// their own, and graphs, which may be replayed on any stream, have none.
+uint64_t* sums_of_stream(hipStream_t stream, int64_t n) {
+  static std::mutex mutex;
+  static auto* all =  // never freed, so not after the runtime's own end
+      new std::map<std::pair<int, hipStream_t>, torch::Tensor>;
+  const int device = c10::hip::current_device();
+  const std::lock_guard<std::mutex> lock(mutex);
+  auto& sums = (*all)[{device, stream}];
+  if (!sums.defined() || sums.numel() < n)
+    sums = torch::full(
+        {std::max<int64_t>(2 * n, 4096)}, -1,
+        torch::TensorOptions().dtype(at::kLong).device(at::kCUDA, device));
+  return reinterpret_cast<uint64_t*>(sums.data_ptr<int64_t>());
+}
+
+bool is_capturing(hipStream_t stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  C10_HIP_CHECK(hipStreamIsCapturing(stream, &status));
+  return status != hipStreamCaptureStatusNone;
+}
+
+// A list's norm on its way: the sums (or largest magnitudes) of n parts, all
+// of which make it up; n is 1 once they are joined, and then `norm` is written.
+struct NormParts {
+  torch::Tensor buffer;  // the parts and, behind them, room for one
+  const double* parts;
+  int64_t n;
+  bool written;
+};
+
+NormParts norm_parts(const Gradients& grads, bool inf, float* norm,
+                     hipStream_t stream) {
+  int64_t n = 0;
+  for (const auto& g : grads.groups()) n += grad_norm_partials(g.spans, g.type);
+  NormParts out;
+  out.buffer = torch::empty(
+      {n + 1}, torch::TensorOptions().dtype(at::kDouble).device(grads.device()));
+  double* parts = out.buffer.data_ptr<double>();
+  uint64_t* sums =
+      n == 0 || is_capturing(stream) ? nullptr : sums_of_stream(stream, n);
+  int64_t at = 0;
+  for (const auto& g : grads.groups())
+    at += launch_grad_norm_partial(g.spans, g.type, inf, parts, at, n, sums,
+                                   parts + n, norm, stream);
+  out.written = sums != nullptr;
+  out.parts = out.written ? parts + n : parts;
+  out.n = out.written ? 1 : n;
+  return out;
 }
 
 torch::Tensor grad_norm(const pybind11::list& list, bool inf) {
@@ -256,10 +301,11 @@ torch::Tensor grad_norm(const pybind11::list& list, bool inf) {
   const Gradients grads(tensors, what, false);
   const c10::DeviceGuard guard(grads.device());
   const auto stream = at::hip::getCurrentHIPStream();
-  const auto partial = norm_partials(grads, inf, stream);
   auto norm = one_float(grads.device());
-  launch_grad_norm_finish(partial.data_ptr<double>(), partial.numel(), inf,
-                          norm.data_ptr<float>(), stream);
+  float* out = norm.data_ptr<float>();
+  const auto parts = norm_parts(grads, inf, out, stream);
+  if (!parts.written)
+    launch_grad_norm_finish(parts.parts, parts.n, inf, out, stream);
   C10_HIP_CHECK(hipGetLastError());
   return norm;
 }
@@ -274,24 +320,23 @@ torch::Tensor grad_clip_norm(const pybind11::list& list, double max_norm,
   const Gradients grads(tensors, what, true);
   const c10::DeviceGuard guard(grads.device());
   const auto stream = at::hip::getCurrentHIPStream();
-  auto partial = norm_partials(grads, inf, stream);
-  const double* sums = partial.data_ptr<double>();
-  int64_t n = partial.numel();
   auto norm = one_float(grads.device());
-  torch::Tensor joined;
-  if (n > kMaxJoinedPartials || n == 0) {
-    // too many for every block of the scaling pass to join them: it gets one
-    joined = torch::empty({1}, partial.options());
-    launch_grad_norm_join(sums, n, inf, joined.data_ptr<double>(), stream);
-    sums = joined.data_ptr<double>();
-    n = 1;
-  }
   float* out = norm.data_ptr<float>();
-  if (grads.groups().empty())
-    launch_grad_norm_finish(sums, n, inf, out, stream);
+  auto parts = norm_parts(grads, inf, out, stream);
+  if (!parts.written && (parts.n > kMaxJoinedPartials || parts.n == 0)) {
+    // too many for every block of the scaling pass to join them
+    double* joined = parts.buffer.data_ptr<double>() + parts.n;
+    launch_grad_norm_join(parts.parts, parts.n, inf, joined, stream);
+    parts.parts = joined;
+    parts.n = 1;
+  }
+  if (!parts.written && grads.groups().empty())
+    launch_grad_norm_finish(parts.parts, parts.n, inf, out, stream);
+  bool write = !parts.written;  // by the first scaling launch
   for (const auto& g : grads.groups()) {
-    launch_grad_scale(g.spans, g.type, inf, sums, n, max_norm, out, stream);
-    out = nullptr;  // the first launch writes the norm
+    launch_grad_scale(g.spans, g.type, inf, parts.parts, parts.n, max_norm,
+                      write ? out : nullptr, stream);
+    write = false;
   }
   C10_HIP_CHECK(hipGetLastError());
   grads.write_copies_back();
