@@ -71,28 +71,45 @@ struct LargestMagnitude {
   }
 };
 
-// The part of a span that one block works on.
+// The part of a span that one block works on: `data` begins at a line's start,
+// elements [begin, end) of it are the block's.
 template <typename T>
 struct Chunk {
+  static constexpr uint32_t kLen = Pack<T>::kLen;
   T* data;
-  uint32_t packs, n;  // whole packs, elements
+  uint32_t begin, end;
 
   __device__ __forceinline__ Chunk(const SpanTable& table, int c) {
     const int s = span_of_chunk(table.first, table.count, c);
-    const uint32_t begin = uint32_t(c - table.first[s]) * table.chunk;
-    const uint32_t left = table.len[s] - begin;
-    n = left < table.chunk ? left : table.chunk;
-    packs = n / Pack<T>::kLen;
-    data = static_cast<T*>(table.ptr[s]) + begin;
+    T* span = reinterpret_cast<T*>(table.base) + table.offset[s];
+    const uint32_t before = line_offset(span);
+    const uint32_t at = uint32_t(c - table.first[s]) * table.chunk;
+    const uint32_t stop = before + table.len[s] - at;
+    data = span - before + at;
+    begin = at == 0 ? before : 0;
+    end = stop < table.chunk ? stop : table.chunk;
+  }
+
+  // f(i) for the packs of this thread, four at a time where there are as many
+  // (f4), and g(i) for single elements before the first and behind the last.
+  template <typename F4, typename F, typename G>
+  __device__ __forceinline__ void each(F4 f4, F f, G g) const {
+    const uint32_t first = (begin + kLen - 1) / kLen, last = end / kLen;
+    uint32_t i = threadIdx.x + (threadIdx.x < first ? kSpanBlock : 0);
+    for (; i + 3 * kSpanBlock < last; i += 4 * kSpanBlock) f4(i);
+    for (; i < last; i += kSpanBlock) f(i);
+    // the elements of a span within one pack are all behind `last`
+    const uint32_t head = first * kLen < end ? first * kLen : end;
+    const uint32_t tail = last > first ? last * kLen : head;
+    const uint32_t t = threadIdx.x;
+    if (begin + t < head) g(begin + t);
+    if (tail + t < end && t < kLen) g(tail + t);
   }
 };
 
 // Above this size a list does not stay in the 256 MB memory-side cache
 // between two steps.
 constexpr int64_t kCachedBytes = 128 << 20;
-
-// Loads of a thread in flight at a time.
-constexpr int kUnroll = 4;
 
 // The single block that joins all partial results.
 constexpr int kJoinBlock = 1024;
@@ -179,18 +196,16 @@ __global__ __launch_bounds__(kSpanBlock) void grad_norm_partial_kernel(
     #pragma unroll
     for (int j = 0; j < L; ++j) red.add(static_cast<float>(v[j]), j);
   };
-  uint32_t i = threadIdx.x;
-  for (; i + (kUnroll - 1) * kSpanBlock < chunk.packs;
-       i += kUnroll * kSpanBlock) {
-    V v[kUnroll];
-    #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) v[k] = packs[i + k * kSpanBlock];
-    #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) add(v[k]);
-  }
-  for (; i < chunk.packs; i += kSpanBlock) add(packs[i]);
-  const uint32_t t = chunk.packs * L + threadIdx.x;
-  if (t < chunk.n) red.add(static_cast<float>(chunk.data[t]), 0);
+  chunk.each(
+      [&](uint32_t i) {
+        V v[4];
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = packs[i + k * kSpanBlock];
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) add(v[k]);
+      },
+      [&](uint32_t i) { add(packs[i]); },
+      [&](uint32_t i) { red.add(static_cast<float>(chunk.data[i]), 0); });
   const double sum = red.template join<kSpanBlock>(scratch);
   const int own = at + blockIdx.x;
   if (end.sums == nullptr) {
@@ -235,28 +250,27 @@ __device__ __forceinline__ void map_chunk(const Chunk<T>& chunk, F f) {
       v[j] = static_cast<T>(f(static_cast<float>(v[j])));
     return v;
   };
-  uint32_t i = threadIdx.x;
-  for (; i + (kUnroll - 1) * kSpanBlock < chunk.packs;
-       i += kUnroll * kSpanBlock) {
-    V v[kUnroll];
-    #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      V* at = packs + i + k * kSpanBlock;
-      v[k] = kStream ? __builtin_nontemporal_load(at) : *at;
-    }
-    #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      V* at = packs + i + k * kSpanBlock;
-      if (kStream)
-        __builtin_nontemporal_store(map(v[k]), at);
-      else
-        *at = map(v[k]);
-    }
-  }
-  for (; i < chunk.packs; i += kSpanBlock) packs[i] = map(packs[i]);
-  const uint32_t t = chunk.packs * L + threadIdx.x;
-  if (t < chunk.n)
-    chunk.data[t] = static_cast<T>(f(static_cast<float>(chunk.data[t])));
+  chunk.each(
+      [&](uint32_t i) {
+        V v[4];
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          V* at = packs + i + k * kSpanBlock;
+          v[k] = kStream ? __builtin_nontemporal_load(at) : *at;
+        }
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          V* at = packs + i + k * kSpanBlock;
+          if (kStream)
+            __builtin_nontemporal_store(map(v[k]), at);
+          else
+            *at = map(v[k]);
+        }
+      },
+      [&](uint32_t i) { packs[i] = map(packs[i]); },
+      [&](uint32_t i) {
+        chunk.data[i] = static_cast<T>(f(static_cast<float>(chunk.data[i])));
+      });
 }
 
 template <typename T, typename Reduce>
@@ -298,24 +312,32 @@ int64_t chunk_elements(int64_t total, SpanType type) {
 // the tables before) for each and returns the number of all chunks.
 template <typename F>
 int64_t for_tables(const std::vector<TensorSpan>& spans, SpanType type, F f) {
+  const int64_t size = element_size(type);
   int64_t done = 0;
-  for (size_t at = 0; at < spans.size(); at += kMaxSpans) {
+  for (size_t at = 0, next; at < spans.size(); at = next) {
     SpanTable table;
-    table.count =
-        static_cast<int>(std::min<size_t>(kMaxSpans, spans.size() - at));
+    Reach reach;
     int64_t total = 0;
-    for (int i = 0; i < table.count; ++i) total += spans[at + i].len;
+    for (next = at; next < spans.size() && next - at < kMaxSpans; ++next) {
+      if (!reach.fits(spans[next].ptr, size)) break;
+      reach.add(spans[next].ptr);
+      total += spans[next].len;
+    }
+    table.base = reinterpret_cast<char*>(reach.low);
+    table.count = static_cast<int>(next - at);
     const int64_t chunk = chunk_elements(total, type);
     table.chunk = static_cast<uint32_t>(chunk);
-    table.first[0] = 0;
+    int chunks = 0;
     for (int i = 0; i < table.count; ++i) {
       const TensorSpan& s = spans[at + i];
-      table.ptr[i] = s.ptr;
+      const int64_t before =
+          (reinterpret_cast<uintptr_t>(s.ptr) & (kLineBytes - 1)) / size;
+      table.offset[i] = reach.distance(s.ptr, size);
       table.len[i] = static_cast<uint32_t>(s.len);
-      table.first[i + 1] =
-          table.first[i] + static_cast<int>((s.len + chunk - 1) / chunk);
+      table.first[i] = static_cast<uint16_t>(chunks);
+      chunks += static_cast<int>((before + s.len + chunk - 1) / chunk);
     }
-    const int chunks = table.first[table.count];
+    table.first[table.count] = static_cast<uint16_t>(chunks);
     f(table, chunks, done);
     done += chunks;
   }

@@ -55,18 +55,23 @@ struct LambList {
   int* undone;     // whether any chunk is left to the second pass
 };
 
-// A piece of the list as a kernel argument (under 4 KB).
-constexpr int kPieceTensors = 80;
+// A piece of the list as a kernel argument (under 4 KB): each array's tensors
+// by their distance in elements from the lowest of them.
+constexpr int kPieceTensors = 126;
 
 struct LambPiece {
-  float* p[kPieceTensors];
-  const void* g[kPieceTensors];
-  float* m[kPieceTensors];
-  float* v[kPieceTensors];
+  float* p;
+  const char* g;
+  float* m;
+  float* v;
+  uint32_t to_p[kPieceTensors];
+  uint32_t to_g[kPieceTensors];
+  uint32_t to_m[kPieceTensors];
+  uint32_t to_v[kPieceTensors];
   uint32_t len[kPieceTensors];
   int first[kPieceTensors];
   float decay[kPieceTensors];
-  int at, count;
+  int at, count, grad_size;
 };
 
 struct LambRates {
@@ -84,10 +89,10 @@ __global__ __launch_bounds__(kLambBlock) void lamb_list_kernel(
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i < piece.count; i += kLambBlock) {
       const int k = piece.at + i;
-      list.p[k] = piece.p[i];
-      list.g[k] = piece.g[i];
-      list.m[k] = piece.m[i];
-      list.v[k] = piece.v[i];
+      list.p[k] = piece.p + piece.to_p[i];
+      list.g[k] = piece.g + size_t(piece.to_g[i]) * piece.grad_size;
+      list.m[k] = piece.m + piece.to_m[i];
+      list.v[k] = piece.v + piece.to_v[i];
       list.len[k] = piece.len[i];
       list.first[k] = piece.first[i];
       list.decay[k] = piece.decay[i];
@@ -149,25 +154,67 @@ __device__ __forceinline__ bool join_sums(const uint64_t* sums, int c0, int c1,
   return all;
 }
 
+// The part of a tensor that one block works on, cut at multiples of the
+// chunk's size from the line that its parameter begins in.  Pointers are to
+// that place in each array; elements [begin, end) are the block's.
+struct LambChunk {
+  int tensor, c0, c1;  // and the tensor's chunks
+  uint32_t begin, end;
+  uint32_t first, last;  // whole packs
+  uint32_t edge;  // this thread's single element before or behind, or kNone
+  static constexpr uint32_t kNone = ~0u;
+  float *p, *m, *v;
+  const void* g;
+  float decay;
+
+  __device__ __forceinline__ LambChunk(const LambList& list, int c,
+                                       int grad_size) {
+    const int s = span_of_chunk(list.first, list.count, c);
+    tensor = s;
+    c0 = list.first[s];
+    c1 = list.first[s + 1];
+    const uint32_t before = line_offset(list.p[s]);
+    const uint32_t at = uint32_t(c - c0) * kLambChunk;
+    const uint32_t stop = before + list.len[s] - at;
+    begin = at == 0 ? before : 0;
+    end = stop < kLambChunk ? stop : kLambChunk;
+    const int64_t move = int64_t(at) - before;
+    p = list.p[s] + move;
+    m = list.m[s] + move;
+    v = list.v[s] + move;
+    g = static_cast<const char*>(list.g[s]) + move * grad_size;
+    decay = list.decay[s];
+    first = (begin + 3) / 4;
+    last = end / 4;
+    // before the first pack (threads 0 to 3), behind the last (4 to 7)
+    const uint32_t head = first * 4 < end ? first * 4 : end;
+    const uint32_t tail = last > first ? last * 4 : head;
+    const uint32_t t = threadIdx.x;
+    const uint32_t e = t < 4 ? begin + t : tail + t - 4;
+    edge = t < 8 && e < (t < 4 ? head : end) ? e : kNone;
+  }
+  __device__ __forceinline__ bool whole() const {
+    return begin == 0 && end == kLambChunk;
+  }
+  __device__ __forceinline__ bool has(uint32_t pack) const {
+    return pack >= first && pack < last;
+  }
+};
+
 template <typename G>
 __global__ __launch_bounds__(
     kLambBlock, kBlocksPerCu * kLambBlock / (4 * WAVE_SIZE)) void lamb_step_kernel(
     const LambList list, LambRates r, const float* __restrict__ norm,
     double max_norm, uint64_t wait_ticks) {
   __shared__ Pack4 kept[kLdsPacks * kLambBlock];
+  __shared__ float2 edge[8];  // p and u of single elements
   __shared__ double scratch[kLambBlock / WAVE_SIZE];
   typedef G PackG __attribute__((ext_vector_type(4), aligned(sizeof(G))));
   const int c = blockIdx.x;
-  const int s = span_of_chunk(list.first, list.count, c);
-  const int c0 = list.first[s], c1 = list.first[s + 1];
-  const uint32_t begin = uint32_t(c - c0) * kLambChunk;
-  const uint32_t left = list.len[s] - begin;
-  const uint32_t n = left < kLambChunk ? left : kLambChunk;
-  const float decay = list.decay[s];
-  float* p = list.p[s] + begin;
-  const G* g = static_cast<const G*>(list.g[s]) + begin;
-  float* m = list.m[s] + begin;
-  float* v = list.v[s] + begin;
+  const LambChunk chunk(list, c, sizeof(G));
+  const float decay = chunk.decay;
+  float *p = chunk.p, *m = chunk.m, *v = chunk.v;
+  const G* g = static_cast<const G*>(chunk.g);
   float factor = 1.f;
   if (norm != nullptr) {
     const double f = max_norm / (static_cast<double>(*norm) + 1e-6);
@@ -184,7 +231,6 @@ __global__ __launch_bounds__(
     uu = fma(ud, ud, uu);
     return u;
   };
-  const uint32_t nv = n / 4;
   Pack4 u[kPacks], last[kPacks - kLdsPacks];
   auto pack = [&](int k) {
     const uint32_t i = threadIdx.x + k * kLambBlock;
@@ -210,23 +256,24 @@ __global__ __launch_bounds__(
     else
       last[k - kLdsPacks] = pv;
   };
-  float tail_u = 0.f, tail_p = 0.f;
-  const uint32_t t = nv * 4 + threadIdx.x;
-  if (n == kLambChunk) {
+  if (chunk.whole()) {
     #pragma unroll
     for (int k = 0; k < kPacks; ++k) pack(k);
   } else {
     #pragma unroll
     for (int k = 0; k < kPacks; ++k)
-      if (threadIdx.x + k * kLambBlock < nv) pack(k);
-    if (t < n) {
-      float mj = m[t], vj = v[t];
-      tail_p = p[t];
-      tail_u = one(tail_p, static_cast<float>(g[t]), mj, vj);
-      m[t] = mj;
-      v[t] = vj;
+      if (chunk.has(threadIdx.x + k * kLambBlock)) pack(k);
+    if (chunk.edge != LambChunk::kNone) {
+      const uint32_t e = chunk.edge;
+      float mj = m[e], vj = v[e];
+      const float pj = p[e];
+      edge[threadIdx.x] =
+          make_float2(pj, one(pj, static_cast<float>(g[e]), mj, vj));
+      m[e] = mj;
+      v[e] = vj;
     }
   }
+  const int c0 = chunk.c0, c1 = chunk.c1;
   pp = block_sum_f64<kLambBlock>(pp, scratch);
   uu = block_sum_f64<kLambBlock>(uu, scratch);
   if (c1 - c0 > 1) {
@@ -252,14 +299,17 @@ __global__ __launch_bounds__(
     __builtin_nontemporal_store(
         pv, reinterpret_cast<Pack4*>(p) + threadIdx.x + k * kLambBlock);
   };
-  if (n == kLambChunk) {
+  if (chunk.whole()) {
     #pragma unroll
     for (int k = 0; k < kPacks; ++k) update(k);
   } else {
     #pragma unroll
     for (int k = 0; k < kPacks; ++k)
-      if (threadIdx.x + k * kLambBlock < nv) update(k);
-    if (t < n) p[t] = fmaf(step, tail_u, tail_p);
+      if (chunk.has(threadIdx.x + k * kLambBlock)) update(k);
+    if (chunk.edge != LambChunk::kNone) {
+      const float2 d = edge[threadIdx.x];
+      p[chunk.edge] = fmaf(step, d.y, d.x);
+    }
   }
   if (threadIdx.x == 0) list.done[c] = 1;
 }
@@ -286,15 +336,11 @@ __global__ __launch_bounds__(kLambBlock) void lamb_rest_kernel(
   if (*list.undone == 0) return;
   for (int c = blockIdx.x; c < list.chunks; c += gridDim.x) {
     if (list.done[c]) continue;
-    const int s = span_of_chunk(list.first, list.count, c);
-    const int c0 = list.first[s], c1 = list.first[s + 1];
-    const uint32_t begin = uint32_t(c - c0) * kLambChunk;
-    const uint32_t left = list.len[s] - begin;
-    const uint32_t n = left < kLambChunk ? left : kLambChunk;
-    const float decay = list.decay[s];
-    float* p = list.p[s] + begin;
-    const float* m = list.m[s] + begin;
-    const float* v = list.v[s] + begin;
+    const LambChunk chunk(list, c, 0);
+    const int s = chunk.tensor, c0 = chunk.c0, c1 = chunk.c1;
+    const float decay = chunk.decay;
+    float* p = chunk.p;
+    const float *m = chunk.m, *v = chunk.v;
     double pp, uu;
     if (c1 - c0 > list.max_wait) {
       pp = list.totals[2 * s];
@@ -303,8 +349,8 @@ __global__ __launch_bounds__(kLambBlock) void lamb_rest_kernel(
       join_sums<false>(list.sums, c0, c1, 0, scratch, &pp, &uu);
     }
     const float step = lamb_factor(pp, uu, r.lr);
-    const uint32_t nv = n / 4;
-    for (uint32_t i = threadIdx.x; i < nv; i += kLambBlock) {
+    for (uint32_t i = threadIdx.x; i < chunk.last; i += kLambBlock) {
+      if (i < chunk.first) continue;
       Pack4* at = reinterpret_cast<Pack4*>(p) + i;
       Pack4 pv = __builtin_nontemporal_load(at);
       const Pack4 mv =
@@ -316,8 +362,10 @@ __global__ __launch_bounds__(kLambBlock) void lamb_rest_kernel(
         pv[j] = fmaf(step, lamb_rate(pv[j], mv[j], vv[j], decay, r), pv[j]);
       __builtin_nontemporal_store(pv, at);
     }
-    const uint32_t t = nv * 4 + threadIdx.x;
-    if (t < n) p[t] = fmaf(step, lamb_rate(p[t], m[t], v[t], decay, r), p[t]);
+    if (chunk.edge != LambChunk::kNone) {
+      const uint32_t e = chunk.edge;
+      p[e] = fmaf(step, lamb_rate(p[e], m[e], v[e], decay, r), p[e]);
+    }
   }
 }
 
@@ -334,7 +382,9 @@ int max_wait_chunks() {
   return kBlocksPerCu * cus[device] * 4 / 5;
 }
 
-int64_t chunks_of(int64_t len) { return (len + kLambChunk - 1) / kLambChunk; }
+int64_t chunks_of(const LambTensor& t) {
+  return (line_offset(t.p) + t.len + kLambChunk - 1) / kLambChunk;
+}
 
 // The list's arrays one after the other in `bytes` of workspace.
 LambList lay_out(char* at, int count, int chunks, size_t* bytes) {
@@ -367,7 +417,7 @@ LambList lay_out(char* at, int count, int chunks, size_t* bytes) {
 
 int64_t lamb_chunks(const std::vector<LambTensor>& tensors) {
   int64_t n = 0;
-  for (const LambTensor& t : tensors) n += chunks_of(t.len);
+  for (const LambTensor& t : tensors) n += chunks_of(t);
   return n;
 }
 
@@ -406,20 +456,38 @@ void launch_lamb_step(std::vector<LambTensor>& tensors, int64_t chunks,
   const dim3 block(kLambBlock);
   bool long_tensors = false;
   int first = 0;
-  for (int at = 0; at < count; at += kPieceTensors) {
+  const int grad_size = element_size(type);
+  for (int at = 0, next; at < count; at = next) {
+    Reach p, g, m, v;
+    for (next = at; next < count && next - at < kPieceTensors; ++next) {
+      const LambTensor& t = tensors[next];
+      // all four, or none of them
+      if (!p.fits(t.p, 4) || !g.fits(t.g, grad_size) || !m.fits(t.m, 4) ||
+          !v.fits(t.v, 4))
+        break;
+      p.add(t.p);
+      g.add(t.g);
+      m.add(t.m);
+      v.add(t.v);
+    }
     LambPiece piece;
+    piece.p = reinterpret_cast<float*>(p.low);
+    piece.g = reinterpret_cast<const char*>(g.low);
+    piece.m = reinterpret_cast<float*>(m.low);
+    piece.v = reinterpret_cast<float*>(v.low);
     piece.at = at;
-    piece.count = std::min(kPieceTensors, count - at);
+    piece.count = next - at;
+    piece.grad_size = grad_size;
     for (int i = 0; i < piece.count; ++i) {
       const LambTensor& t = tensors[at + i];
-      piece.p[i] = t.p;
-      piece.g[i] = t.g;
-      piece.m[i] = t.m;
-      piece.v[i] = t.v;
+      piece.to_p[i] = p.distance(t.p, 4);
+      piece.to_g[i] = g.distance(t.g, grad_size);
+      piece.to_m[i] = m.distance(t.m, 4);
+      piece.to_v[i] = v.distance(t.v, 4);
       piece.len[i] = static_cast<uint32_t>(t.len);
       piece.first[i] = first;
       piece.decay[i] = t.decay;
-      const int own = static_cast<int>(chunks_of(t.len));
+      const int own = static_cast<int>(chunks_of(t));
       first += own;
       long_tensors = long_tensors || own > list.max_wait;
     }

@@ -342,6 +342,50 @@ def test_tensors_past_32_bits():
 
 
 @pytest.mark.gpu
+def test_tensors_far_apart():
+    """More than 2^32 elements between two tensors of a list."""
+    arena = torch.empty(2 ** 32 + 4096, dtype=torch.bfloat16, device="cuda")
+    far = [arena[3:2003], arena[-777:], arena[5000:5001]]
+    for i, g in enumerate(far):
+        g.copy_(torch.randn(g.shape) * (i + 1))
+    before = [g.clone() for g in far]
+    want = exact_norm(far, 2.0)
+    check_norm(ops.clip_grads_by_norm_(far, want / 9), want)
+    for g, b in zip(far, before):
+        check_scaled(g, b, want, want / 9)
+    ops.clip_grads_by_value_(far, 0.01)
+    assert max(g.abs().max().item() for g in far) <= 0.01 * (1 + 2.0 ** -8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_alignment(dtype):
+    """Each place in a cache line, lengths around it, and chunks that begin
+    inside a tensor; nothing beside the tensors changes."""
+    for n in (1, 2, 7, 8, 9, 63, 64, 65, 129, 4096, 9001):
+        arena = torch.full((40 * (n + 71) + 200,), 7.0, dtype=dtype,
+                           device="cuda")
+        grads, at = [], 0
+        for i in range(40):
+            at += 1 + i % 3
+            grads.append(arena[at:at + n])
+            at += n + 2 * i
+        for i, g in enumerate(grads):
+            g.copy_((torch.randn(n) + 3) * (1 + i % 2))
+        before = [g.clone() for g in grads]
+        rest = outside(arena, grads)
+        want = exact_norm(grads, 2.0)
+        check_norm(ops.clip_grads_by_norm_(grads, want / 2), want)
+        for g, b in zip(grads, before):
+            check_scaled(g, b, want, want / 2)
+        check_norm(ops.global_grad_norm(grads, math.inf),
+                   exact_norm(grads, math.inf))
+        ops.clip_grads_by_value_(grads, 0.25)
+        assert all(g.abs().max().item() <= 0.25 for g in grads)
+        assert torch.equal(outside(arena, grads), rest)
+
+
+@pytest.mark.gpu
 def test_two_streams():
     """Two calls at once, on streams of their own, share nothing."""
     lists = [make([500_001, 77, 3000], torch.float32, "cuda", seed=s, gap=1)[1]

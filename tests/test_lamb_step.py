@@ -143,6 +143,28 @@ def test_large_lists(sizes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("wait_ticks", [0, 20000])
+def test_every_alignment(wait_ticks):
+    """Each place in a cache line, lengths around it and around a block's
+    share; parameters aligned unlike their moments."""
+    for n in (1, 2, 3, 4, 5, 31, 32, 33, 32767, 32768, 32769, 70_000):
+        sizes = [n + i for i in range(9)] * 3
+        arenas, lists = make(sizes, "cuda", gap=3)
+        moved = [torch.empty(sum(sizes) + 40, device="cuda") for _ in "gm"]
+        for k, buffer in zip((1, 2), moved):  # gradients and exp_avgs moved
+            at = 2 * k
+            for i, t in enumerate(lists[k]):
+                lists[k][i] = buffer[at:at + t.numel()].copy_(t)
+                at += t.numel()
+        before = [[t.clone() for t in ts] for ts in lists]
+        ops.extension().lamb_step(*lists, [0.01] * len(sizes), 3, 0.1, B1, B2,
+                                  1e-6, 0.0, None, wait_ticks)
+        check(lists, before, 3, 0.1, 1e-6, [0.01] * len(sizes))
+        for a in (arenas[0], arenas[3]):
+            assert int((a == 7).sum()) >= 3 * (len(sizes) + 1)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("wait_ticks", [0, 1, 1000])
 def test_second_pass_gives_the_same_bits(dtype, wait_ticks):
@@ -371,6 +393,20 @@ def test_two_streams():
     for lists, b in zip(made, before):
         norm = torch.cat([g.cpu().double() for g in b[1]]).norm().item()
         check(lists, b, 5, 0.1, 1e-6, [0.0, 0.0], 1.0 / (norm + 1e-6))
+
+
+@pytest.mark.gpu
+def test_gradients_far_apart():
+    """More than 2^32 elements between the gradients of two parameters."""
+    sizes = [2000, 40_000, 7]
+    _, lists = make(sizes, "cuda", torch.bfloat16, gap=1)
+    arena = torch.empty(2 ** 32 + 100_000, dtype=torch.bfloat16,
+                        device="cuda")
+    for i, at in enumerate((5, 2 ** 32 + 50_000, 3000)):
+        lists[1][i] = arena[at:at + sizes[i]].copy_(lists[1][i])
+    before = [[t.clone() for t in ts] for ts in lists]
+    ops.fused_lamb_step(*lists, step=2, lr=0.1)
+    check(lists, before, 2, 0.1, 1e-6, [0.0] * 3)
 
 
 @pytest.mark.gpu
