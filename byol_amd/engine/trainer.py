@@ -210,13 +210,15 @@ def execute_graph(epoch, model, loader, grapher, args, optimizer=None,
 
     from ..ops.classifier import cross_entropy_topk
 
+    parameters = list(model.parameters())
+    clip_norm = getattr(args, "clip_norm", 0.0)
+
     def clip_gradients():
         if args.clip > 0:
-            clip_grad_value_(model.parameters(), args.clip)
-        clip_norm = getattr(args, "clip_norm", 0.0)
+            clip_grad_value_(parameters, args.clip)
         # LAMB clips by norm while it reads the gradients
         if clip_norm > 0 and not getattr(optimizer, "max_grad_norm", 0.0):
-            clip_grad_norm_(model.parameters(), clip_norm)
+            clip_grad_norm_(parameters, clip_norm)
 
     def train_step_body(a1, a2, lab):
         """One full training step (fwd + losses + bwd + opt) — runs eager

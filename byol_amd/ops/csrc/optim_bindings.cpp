@@ -360,6 +360,40 @@ void grad_clip_value(const pybind11::list& list, double clip_value) {
   mark_written(tensors);
 }
 
+// Whether lamb_step takes these lists together, types, layouts and devices
+// being what they are; it still refuses tensors that share memory.
+bool lamb_fits(const pybind11::list& param_list,
+               const pybind11::list& grad_list,
+               const pybind11::list& exp_avg_list,
+               const pybind11::list& exp_avg_sq_list) {
+  const char* what = "lamb_fits";
+  const TensorList params(param_list, what), grads(grad_list, what),
+      exp_avgs(exp_avg_list, what), exp_avg_sqs(exp_avg_sq_list, what);
+  const size_t n = params.size();
+  if (n == 0 || grads.size() != n || exp_avgs.size() != n ||
+      exp_avg_sqs.size() != n)
+    return false;
+  const auto device = params[0].device();
+  const auto grad_type = grads[0].scalar_type();
+  if (!device.is_cuda() ||
+      (grad_type != at::kFloat && grad_type != at::kBFloat16 &&
+       grad_type != at::kHalf))
+    return false;
+  for (size_t i = 0; i < n; ++i) {
+    const auto &p = params[i], &g = grads[i];
+    if (p.numel() >= (int64_t(1) << 31) || g.device() != device ||
+        g.layout() != at::kStrided || g.scalar_type() != grad_type ||
+        g.sizes() != p.sizes())
+      return false;
+    for (const auto* t : {&p, &exp_avgs[i], &exp_avg_sqs[i]})
+      if (t->layout() != at::kStrided || t->scalar_type() != at::kFloat ||
+          t->device() != device || !t->is_non_overlapping_and_dense() ||
+          t->sizes() != p.sizes() || !same_layout(*t, p))
+        return false;
+  }
+  return true;
+}
+
 void lamb_step(const pybind11::list& param_list,
                const pybind11::list& grad_list,
                const pybind11::list& exp_avg_list,
@@ -460,6 +494,7 @@ void bind_optim(pybind11::module& mod) {
           "clip gradients by their global norm (gfx950)");
   mod.def("grad_clip_value", &grad_clip_value,
           "clip gradients by value (gfx950)");
+  mod.def("lamb_fits", &lamb_fits, "whether lamb_step takes these lists");
   mod.def("lamb_step", &lamb_step, "multi-tensor LAMB step (gfx950)",
           pybind11::arg("params"), pybind11::arg("grads"),
           pybind11::arg("exp_avgs"), pybind11::arg("exp_avg_sqs"),

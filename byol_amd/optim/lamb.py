@@ -61,39 +61,26 @@ class LAMB(Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        norm = None
-        if self.max_grad_norm > 0:
-            from ..ops import global_grad_norm
-            grads = [p.grad for group in self.param_groups
-                     for p in group["params"] if p.grad is not None]
-            if grads:
-                norm = global_grad_norm(grads)
-        fused = {}
+        groups = []
         for group in self.param_groups:
-            key = (group["lr"], tuple(group["betas"]), group["eps"])
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
-                state = self.state[p]
-                if len(state) == 0:
-                    state["step"] = 0
-                    state["exp_avg"] = torch.zeros_like(p)
-                    state["exp_avg_sq"] = torch.zeros_like(p)
+            params = [p for p in group["params"] if p.grad is not None]
+            if params:
+                groups.append((group, params, [p.grad for p in params]))
+        norm = None
+        if self.max_grad_norm > 0 and groups:
+            from ..ops import global_grad_norm
+            norm = global_grad_norm([g for _, _, gs in groups for g in gs])
+        fused = {}
+        for group, params, grads in groups:
+            states = [self._state_of(p) for p in params]
+            for state in states:
                 state["step"] += 1
-                if not _takes_fused_step(p):
-                    self._step_one(p, state, group, norm)
-                    continue
-                for name in ("exp_avg", "exp_avg_sq"):
-                    # a checkpoint of another memory format
-                    if state[name].stride() != p.stride():
-                        state[name] = torch.empty_like(p).copy_(state[name])
-                lists = fused.setdefault(
-                    (p.device, p.grad.dtype, state["step"], *key),
-                    ([], [], [], [], []))
-                for values, value in zip(lists, (
-                        p, p.grad, state["exp_avg"], state["exp_avg_sq"],
-                        max(group["weight_decay"], 0.0))):
-                    values.append(value)
+            lists = (params, grads, [s["exp_avg"] for s in states],
+                     [s["exp_avg_sq"] for s in states])
+            if params[0].is_cuda and self._fit_one_step(lists, states):
+                self._add_to_step(fused, group, lists, states[0]["step"])
+            else:
+                self._step_each(fused, group, params, states, norm)
         if fused:
             from ..ops import fused_lamb_step
             for (_, _, step, lr, betas, eps), lists in fused.items():
@@ -102,6 +89,45 @@ class LAMB(Optimizer):
                                 max_grad_norm=self.max_grad_norm,
                                 grad_norm=norm)
         return loss
+
+    def _state_of(self, p):
+        state = self.state[p]
+        if len(state) == 0:
+            state["step"] = 0
+            state["exp_avg"] = torch.zeros_like(p)
+            state["exp_avg_sq"] = torch.zeros_like(p)
+        return state
+
+    @staticmethod
+    def _fit_one_step(lists, states) -> bool:
+        """Whether a group's tensors can all go into the same fused step."""
+        from ..ops import require_extension
+        return require_extension("LAMB.step").lamb_fits(*lists) \
+            and len({s["step"] for s in states}) == 1
+
+    @staticmethod
+    def _add_to_step(fused, group, lists, step):
+        params, grads = lists[:2]
+        key = (params[0].device, grads[0].dtype, step, group["lr"],
+               tuple(group["betas"]), group["eps"])
+        all_lists = fused.setdefault(key, ([], [], [], [], []))
+        for values, more in zip(all_lists, lists):
+            values.extend(more)
+        all_lists[4].extend([max(group["weight_decay"], 0.0)] * len(params))
+
+    def _step_each(self, fused, group, params, states, norm):
+        for p, state in zip(params, states):
+            if not _takes_fused_step(p):
+                self._step_one(p, state, group, norm)
+                continue
+            for name in ("exp_avg", "exp_avg_sq"):
+                # a checkpoint of another memory format or type
+                if state[name].stride() != p.stride() \
+                        or state[name].dtype != p.dtype:
+                    state[name] = torch.empty_like(p).copy_(state[name])
+            self._add_to_step(fused, group,
+                              ([p], [p.grad], [state["exp_avg"]],
+                               [state["exp_avg_sq"]]), state["step"])
 
     def _step_one(self, p, state, group, norm):
         beta1, beta2 = group["betas"]
