@@ -13,8 +13,10 @@ as one tensor.  Elsewhere the same values come from elementary torch
 operations, the oracle of the tests.
 
 Gradients are fp32, bf16 or fp16, types may differ within a list; strided
-tensors are taken as they are.  NaN and infinities propagate: an infinite norm
-scales finite gradients to zero, a NaN norm makes all of them NaN.
+tensors are taken as they are.  Tensors that are written must not overlap:
+their ranges of memory, also where views interleave, have to be apart.  NaN and
+infinities propagate: an infinite norm scales finite gradients to zero, a NaN
+norm makes all of them NaN.  Nothing here is differentiated through.
 """
 
 import math
@@ -37,19 +39,26 @@ def _is_inf(norm_type: float) -> bool:
     return norm_type == math.inf
 
 
+def _as_list(grads) -> list:
+    return [grads] if isinstance(grads, torch.Tensor) else list(grads)
+
+
 def _on_gpu(grads: Sequence[torch.Tensor], what: str) -> bool:
     """Whether the HIP kernels take the list (their binding then checks it);
     a list on the CPU is checked here."""
-    if grads[0].is_cuda or any(t.is_cuda for t in grads):
+    if getattr(grads[0], "is_cuda", False) \
+            or any(getattr(t, "is_cuda", False) for t in grads):
         return True
     for t in grads:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: expected tensors, got {type(t)}")
         if t.dtype not in _DTYPES or t.layout is not torch.strided:
             raise TypeError(f"{what}: expected dense fp32, bf16 or fp16 "
                             f"tensors, got {t.dtype} ({t.layout})")
     return False
 
 
-def _check_writable(grads: Sequence[torch.Tensor], what: str) -> None:
+def check_writable(grads: Sequence[torch.Tensor], what: str) -> None:
     ranges = []
     for t in grads:
         if t.numel() == 0:
@@ -81,7 +90,7 @@ def global_grad_norm(grads: Sequence[torch.Tensor],
     elements of all tensors, as one fp32 value on their device.  An empty
     list has norm 0."""
     inf = _is_inf(norm_type)
-    grads = list(grads)
+    grads = _as_list(grads)
     if not grads:
         return torch.zeros(())
     if _on_gpu(grads, "global_grad_norm"):
@@ -99,13 +108,13 @@ def clip_grads_by_norm_(grads: Sequence[torch.Tensor], max_norm: float,
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
-    grads = list(grads)
+    grads = _as_list(grads)
     if not grads:
         return torch.zeros(())
     what = "clip_grads_by_norm_"
     if _on_gpu(grads, what):
         return require_extension(what).grad_clip_norm(grads, max_norm, inf)
-    _check_writable(grads, what)
+    check_writable(grads, what)
     with torch.no_grad():
         norm = _reference_norm(grads, inf)
         factor = (max_norm / (norm + 1e-6)).clamp(max=1.0).float()
@@ -122,14 +131,14 @@ def clip_grads_by_value_(grads: Sequence[torch.Tensor],
     clip_value = float(clip_value)
     if not clip_value >= 0:
         raise ValueError(f"clip_value must be >= 0, got {clip_value}")
-    grads = list(grads)
+    grads = _as_list(grads)
     if not grads:
         return
     what = "clip_grads_by_value_"
     if _on_gpu(grads, what):
         require_extension(what).grad_clip_value(grads, clip_value)
         return
-    _check_writable(grads, what)
+    check_writable(grads, what)
     with torch.no_grad():
         for t in grads:
             t.copy_(t.float().clamp(-clip_value, clip_value))

@@ -18,7 +18,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import require_extension
-from .grad_clip import global_grad_norm
+from .grad_clip import check_writable, global_grad_norm
 
 __all__ = ["fused_lamb_step"]
 
@@ -94,6 +94,7 @@ def _reference_step(params, grads, exp_avgs, exp_avg_sqs, decay, step, lr,
         if not p.shape == g.shape == m.shape == v.shape:
             raise ValueError("fused_lamb_step: a gradient or moment has "
                              "another shape than its parameter")
+    check_writable([*params, *exp_avgs, *exp_avg_sqs], "fused_lamb_step")
     factor = 1.0
     if grad_norm is not None:
         factor = (max_grad_norm / (grad_norm.double() + 1e-6)) \

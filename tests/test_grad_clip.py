@@ -226,6 +226,18 @@ def test_nothing_to_clip(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_one_tensor_is_a_list_of_it(device):
+    g = torch.full((4, 4), 2.0, device=device)
+    check_norm(ops.global_grad_norm(g), 8.0)
+    check_norm(ops.clip_grads_by_norm_(g, 4.0), 8.0)
+    check_scaled(g, torch.full((4, 4), 2.0), 8.0, 4.0)
+    ops.clip_grads_by_value_(g, 0.5)
+    assert (g == 0.5).all()
+    with pytest.raises(TypeError):
+        ops.global_grad_norm([1.0, g])
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_refusals(device):
     g = torch.ones(64, device=device)
     calls = [lambda t: ops.clip_grads_by_norm_(t, 0.1),

@@ -20,9 +20,12 @@ the small sizes where it is tested.  1.01 covers products of these terms.
 """
 
 import math
+import os
 
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 from byol_amd import ops
 from byol_amd.optim.lamb import LAMB
@@ -237,6 +240,8 @@ def test_refusals(device):
         ops.fused_lamb_step(p, g, m[:1], v, step=1, lr=0.1)
     with pytest.raises(ValueError, match="shape"):
         ops.fused_lamb_step(p, [g[0], g[0]], m, v, step=1, lr=0.1)
+    with pytest.raises(ValueError, match="twice"):
+        ops.fused_lamb_step(p, g, m, m, step=1, lr=0.1)
     with pytest.raises(TypeError):
         ops.fused_lamb_step([t.double() for t in p], g, m, v, step=1, lr=0.1)
     with pytest.raises(TypeError):
@@ -474,3 +479,55 @@ def test_engine_epoch(device, extra, tmp_path):
         # the gradients live in the flat buffer still
         model.flat_space.flat_grads.fill_(2.0)
         assert all((p.grad == 2).all() for p in model.parameters())
+
+
+def _replica(rank, port, out_dir, lamb):
+    import types
+
+    from byol_amd.models.byol import BYOL
+    from byol_amd.optim import build_optimizer, clip_grad_norm_
+    from byol_amd.parallel.ddp import FlatDDP
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    torch.manual_seed(rank)  # FlatDDP aligns the parameters
+    model = BYOL(arch="resnet18", base_network_output_size=512,
+                 projection_output_size=8, classifier_output_size=3,
+                 total_training_steps=10, head_latent_size=16).finalize()
+    ddp = FlatDDP(model)
+    opt, _ = build_optimizer(ddp, types.SimpleNamespace(
+        optimizer="lamb" if lamb else "lars_momentum", lr=0.01,
+        weight_decay=1e-4, batch_size=4, num_replicas=2, clip_norm=0.5,
+        lr_update_schedule="fixed", epochs=2, warmup=0))
+    ddp.train()
+    norms = []
+    torch.manual_seed(100 + rank)
+    for _ in range(3):
+        out = ddp(torch.rand(4, 3, 32, 32), torch.rand(4, 3, 32, 32))
+        loss = out["online_prediction1"].square().mean() \
+            + out["linear_preds"].square().mean()
+        opt.zero_grad()
+        loss.backward()
+        ddp.finish_grad_sync()
+        if not lamb:
+            norms.append(clip_grad_norm_(ddp.parameters(), 0.5))
+            norms.append(ops.global_grad_norm([model.flat_space.flat_grads]))
+        opt.step()
+    torch.save({"params": model.flat_space.flat_params, "norms": norms},
+               os.path.join(out_dir, f"{rank}.pt"))
+    dist.destroy_process_group()
+
+
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("lamb", [True, False])
+def test_replicas_stay_alike(lamb, tmp_path):
+    """Two ranks on different data: the clipped steps follow the averaged
+    gradients, the same on both."""
+    mp.spawn(_replica, args=(29561 + lamb, str(tmp_path), lamb), nprocs=2,
+             join=True)
+    a, b = (torch.load(tmp_path / f"{r}.pt", weights_only=True)
+            for r in (0, 1))
+    assert torch.equal(a["params"], b["params"])
+    for x, y in zip(a["norms"], b["norms"]):
+        assert torch.equal(x, y)
+    assert all(n <= 0.5 * (1 + 4 * E) for n in a["norms"][1::2])
