@@ -237,7 +237,9 @@ def execute_graph(epoch, model, loader, grapher, args, optimizer=None,
                 out["linear_preds"].float().contiguous(),
                 torch.cat([lab, lab], 0))
             total = byol_loss + classifier_loss
-        optimizer.zero_grad()
+        # FlatDDP reduces the flat buffer that the gradients are views of;
+        # dropped, they would come back outside of it
+        optimizer.zero_grad(set_to_none=not is_ddp)
         if scaler.is_enabled():
             scaler.scale(total).backward()
             if is_ddp:

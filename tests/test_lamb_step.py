@@ -481,6 +481,26 @@ def test_engine_epoch(device, extra, tmp_path):
         assert all((p.grad == 2).all() for p in model.parameters())
 
 
+@pytest.mark.parametrize("optimizer", ["lamb", "adam", "lars_momentum"])
+def test_engine_keeps_gradients_where_they_are_reduced(optimizer, tmp_path):
+    from byol_amd.engine import trainer
+    from byol_amd.optim import build_optimizer
+    from byol_amd.parallel.ddp import FlatDDP
+    args = engine_args(tmp_path, "cpu", "--optimizer", optimizer,
+                       "--clip-norm", "1.0")
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", "29571"
+    dist.init_process_group("gloo", rank=0, world_size=1)
+    try:
+        loader, model, grapher = trainer.build_loader_model_grapher(args)
+        ddp = FlatDDP(model)
+        opt, _ = build_optimizer(ddp, args)
+        trainer.train(1, ddp, opt, loader.train_loader, grapher, args)
+    finally:
+        dist.destroy_process_group()
+    model.flat_space.flat_grads.fill_(2.0)
+    assert all((p.grad == 2).all() for p in model.parameters())
+
+
 def _replica(rank, port, out_dir, lamb):
     import types
 
