@@ -308,69 +308,33 @@ int64_t chunk_elements(int64_t total, SpanType type) {
   return std::max(2 * step, (want + step - 1) / step * step);
 }
 
-// The list in tables of at most kMaxSpans; calls f(table, chunks, chunks of
-// the tables before) for each and returns the number of all chunks.
-template <typename F>
-int64_t for_tables(const std::vector<TensorSpan>& spans, SpanType type, F f) {
-  const int64_t size = element_size(type);
-  int64_t done = 0;
-  for (size_t at = 0, next; at < spans.size(); at = next) {
-    SpanTable table;
-    Reach reach;
-    int64_t total = 0;
-    for (next = at; next < spans.size() && next - at < kMaxSpans; ++next) {
-      if (!reach.fits(spans[next].ptr, size)) break;
-      reach.add(spans[next].ptr);
-      total += spans[next].len;
-    }
-    table.base = reinterpret_cast<char*>(reach.low);
-    table.count = static_cast<int>(next - at);
-    const int64_t chunk = chunk_elements(total, type);
-    table.chunk = static_cast<uint32_t>(chunk);
-    int chunks = 0;
-    for (int i = 0; i < table.count; ++i) {
-      const TensorSpan& s = spans[at + i];
-      const int64_t before =
-          (reinterpret_cast<uintptr_t>(s.ptr) & (kLineBytes - 1)) / size;
-      table.offset[i] = reach.distance(s.ptr, size);
-      table.len[i] = static_cast<uint32_t>(s.len);
-      table.first[i] = static_cast<uint16_t>(chunks);
-      chunks += static_cast<int>((before + s.len + chunk - 1) / chunk);
-    }
-    table.first[table.count] = static_cast<uint16_t>(chunks);
-    f(table, chunks, done);
-    done += chunks;
-  }
-  return done;
-}
-
 template <typename Reduce>
-int64_t launch_partials(const std::vector<TensorSpan>& spans, SpanType type,
-                        double* partial, int64_t at, const NormEnd& end,
-                        hipStream_t stream) {
-  return for_tables(spans, type, [&](const SpanTable& t, int chunks,
-                                     int64_t done) {
-    with_element_type(type, [&](auto value) {
+void launch_partials(const SpanGroup& group, double* partial, int64_t at,
+                     const NormEnd& end, hipStream_t stream) {
+  for (const SpanTable& t : group.tables) {
+    const int chunks = t.first[t.count];
+    with_element_type(group.type, [&](auto value) {
       hipLaunchKernelGGL(
           (grad_norm_partial_kernel<decltype(value), Reduce>), dim3(chunks),
-          dim3(kSpanBlock), 0, stream, t, partial,
-          static_cast<int>(at + done), end);
+          dim3(kSpanBlock), 0, stream, t, partial, static_cast<int>(at), end);
     });
-  });
+    at += chunks;
+  }
 }
 
+// The tables, too, in the opposite order of the norm's pass.
 template <typename Reduce>
-void launch_scale(const std::vector<TensorSpan>& spans, SpanType type,
-                  const double* partial, int n, double bound, float* norm,
-                  hipStream_t stream) {
-  for_tables(spans, type, [&](const SpanTable& t, int chunks, int64_t done) {
-    with_element_type(type, [&](auto value) {
+void launch_scale(const SpanGroup& group, const double* partial, int n,
+                  double bound, float* norm, hipStream_t stream) {
+  for (auto t = group.tables.rbegin(); t != group.tables.rend(); ++t) {
+    const int chunks = t->first[t->count];
+    with_element_type(group.type, [&](auto value) {
       hipLaunchKernelGGL((grad_scale_kernel<decltype(value), Reduce>),
                          dim3((chunks + 7) / 8 * 8), dim3(kSpanBlock), 0,
-                         stream, t, partial, n, bound,
-                         done == 0 ? norm : nullptr);
+                         stream, *t, partial, n, bound, norm);
     });
-  });
+    norm = nullptr;  // the first launch writes it
+  }
 }
 
 void launch_finish(const double* partial, int n, bool inf, float* norm,
@@ -385,22 +349,48 @@ void launch_finish(const double* partial, int n, bool inf, float* norm,
 
 }  // namespace
 
-// Partial results that launch_grad_norm_partial writes for this list.
-int64_t grad_norm_partials(const std::vector<TensorSpan>& spans,
-                           SpanType type) {
-  return for_tables(spans, type, [](const SpanTable&, int, int64_t) {});
+// Fills in the tables of a group's spans.
+void make_tables(SpanGroup& group) {
+  const auto& spans = group.spans;
+  const int64_t size = element_size(group.type);
+  for (size_t at = 0, next; at < spans.size(); at = next) {
+    Reach reach;
+    int64_t total = 0;
+    for (next = at; next < spans.size() && next - at < kMaxSpans; ++next) {
+      if (!reach.fits(spans[next].ptr, size)) break;
+      reach.add(spans[next].ptr);
+      total += spans[next].len;
+    }
+    group.tables.emplace_back();
+    SpanTable& table = group.tables.back();
+    table.base = reinterpret_cast<char*>(reach.low);
+    table.count = static_cast<int>(next - at);
+    const int64_t chunk = chunk_elements(total, group.type);
+    table.chunk = static_cast<uint32_t>(chunk);
+    int chunks = 0;
+    for (int i = 0; i < table.count; ++i) {
+      const TensorSpan& s = spans[at + i];
+      const int64_t before =
+          (reinterpret_cast<uintptr_t>(s.ptr) & (kLineBytes - 1)) / size;
+      table.offset[i] = reach.distance(s.ptr, size);
+      table.len[i] = static_cast<uint32_t>(s.len);
+      table.first[i] = static_cast<uint16_t>(chunks);
+      chunks += static_cast<int>((before + s.len + chunk - 1) / chunk);
+    }
+    table.first[table.count] = static_cast<uint16_t>(chunks);
+  }
 }
 
-int64_t launch_grad_norm_partial(const std::vector<TensorSpan>& spans,
-                                 SpanType type, bool inf, double* partial,
-                                 int64_t at, int64_t all, uint64_t* sums,
-                                 double* joined, float* norm,
-                                 hipStream_t stream) {
+// Writes one partial result for each chunk, from partial[at] on.
+void launch_grad_norm_partial(const SpanGroup& group, bool inf,
+                              double* partial, int64_t at, int64_t all,
+                              uint64_t* sums, double* joined, float* norm,
+                              hipStream_t stream) {
   const NormEnd end = {sums, static_cast<int>(all), joined, norm};
-  return inf ? launch_partials<LargestMagnitude>(spans, type, partial, at, end,
-                                                 stream)
-             : launch_partials<SumOfSquares>(spans, type, partial, at, end,
-                                             stream);
+  if (inf)
+    launch_partials<LargestMagnitude>(group, partial, at, end, stream);
+  else
+    launch_partials<SumOfSquares>(group, partial, at, end, stream);
 }
 
 void launch_grad_norm_finish(const double* partial, int64_t n, bool inf,
@@ -413,26 +403,26 @@ void launch_grad_norm_join(const double* partial, int64_t n, bool inf,
   launch_finish(partial, static_cast<int>(n), inf, nullptr, joined, stream);
 }
 
-void launch_grad_scale(const std::vector<TensorSpan>& spans, SpanType type,
-                       bool inf, const double* partial, int64_t n,
-                       double bound, float* norm, hipStream_t stream) {
+void launch_grad_scale(const SpanGroup& group, bool inf,
+                       const double* partial, int64_t n, double bound,
+                       float* norm, hipStream_t stream) {
   if (inf)
-    launch_scale<LargestMagnitude>(spans, type, partial, static_cast<int>(n),
-                                   bound, norm, stream);
+    launch_scale<LargestMagnitude>(group, partial, static_cast<int>(n), bound,
+                                   norm, stream);
   else
-    launch_scale<SumOfSquares>(spans, type, partial, static_cast<int>(n),
-                               bound, norm, stream);
+    launch_scale<SumOfSquares>(group, partial, static_cast<int>(n), bound,
+                               norm, stream);
 }
 
-void launch_grad_clamp(const std::vector<TensorSpan>& spans, SpanType type,
-                       float bound, hipStream_t stream) {
+void launch_grad_clamp(const SpanGroup& group, float bound,
+                       hipStream_t stream) {
   int64_t total = 0;
-  for (const TensorSpan& s : spans) total += s.len;
-  const bool streamed = total * element_size(type) > kCachedBytes;
-  for_tables(spans, type, [&](const SpanTable& t, int chunks, int64_t) {
-    with_element_type(type, [&](auto value) {
+  for (const TensorSpan& s : group.spans) total += s.len;
+  const bool streamed = total * element_size(group.type) > kCachedBytes;
+  for (const SpanTable& t : group.tables) {
+    with_element_type(group.type, [&](auto value) {
       using T = decltype(value);
-      const dim3 grid(chunks), block(kSpanBlock);
+      const dim3 grid(t.first[t.count]), block(kSpanBlock);
       if (streamed)
         hipLaunchKernelGGL((grad_clamp_kernel<T, true>), grid, block, 0,
                            stream, t, bound);
@@ -440,5 +430,5 @@ void launch_grad_clamp(const std::vector<TensorSpan>& spans, SpanType type,
         hipLaunchKernelGGL((grad_clamp_kernel<T, false>), grid, block, 0,
                            stream, t, bound);
     });
-  });
+  }
 }

@@ -52,15 +52,6 @@ struct Reach {
   }
 };
 
-struct SpanTable {
-  char* base;  // the lowest address; offsets are in elements
-  uint32_t offset[kMaxSpans];
-  uint32_t len[kMaxSpans];
-  uint16_t first[kMaxSpans + 1];  // a span's first chunk; [count] = all chunks
-  int count;
-  uint32_t chunk;  // elements, a multiple of kLineBytes
-};
-
 // A span is cut into chunks at multiples of the chunk's size from the cache
 // line that it begins in, so that every access of a wave covers whole lines:
 // stores that share lines cost 15% (152 MB clamped: 66 us for 58 us), loads at

@@ -18,22 +18,20 @@
 
 #include "tensor_span.h"
 
-int64_t grad_norm_partials(const std::vector<TensorSpan>& spans,
-                           SpanType type);
-int64_t launch_grad_norm_partial(const std::vector<TensorSpan>& spans,
-                                 SpanType type, bool inf, double* partial,
-                                 int64_t at, int64_t all, uint64_t* sums,
-                                 double* joined, float* norm,
-                                 hipStream_t stream);
+void make_tables(SpanGroup& group);
+void launch_grad_norm_partial(const SpanGroup& group, bool inf,
+                              double* partial, int64_t at, int64_t all,
+                              uint64_t* sums, double* joined, float* norm,
+                              hipStream_t stream);
 void launch_grad_norm_finish(const double* partial, int64_t n, bool inf,
                              float* norm, hipStream_t stream);
 void launch_grad_norm_join(const double* partial, int64_t n, bool inf,
                            double* joined, hipStream_t stream);
-void launch_grad_scale(const std::vector<TensorSpan>& spans, SpanType type,
-                       bool inf, const double* partial, int64_t n,
-                       double bound, float* norm, hipStream_t stream);
-void launch_grad_clamp(const std::vector<TensorSpan>& spans, SpanType type,
-                       float bound, hipStream_t stream);
+void launch_grad_scale(const SpanGroup& group, bool inf,
+                       const double* partial, int64_t n, double bound,
+                       float* norm, hipStream_t stream);
+void launch_grad_clamp(const SpanGroup& group, float bound,
+                       hipStream_t stream);
 int64_t lamb_chunks(const std::vector<LambTensor>& tensors);
 int64_t lamb_workspace_bytes(int64_t count, int64_t chunks);
 void launch_lamb_step(std::vector<LambTensor>& tensors, int64_t chunks,
@@ -188,13 +186,10 @@ class Gradients {
         add(copies_.back().second, types[i]);
       }
     }
+    for (SpanGroup& g : groups_) make_tables(g);
   }
 
-  struct Group {
-    SpanType type;
-    std::vector<TensorSpan> spans;
-  };
-  const std::vector<Group>& groups() const { return groups_; }
+  const std::vector<SpanGroup>& groups() const { return groups_; }
   const torch::Device& device() const { return device_; }
 
   void write_copies_back() const {
@@ -203,11 +198,11 @@ class Gradients {
 
  private:
   void add(const torch::Tensor& t, SpanType type) {
-    Group* group = nullptr;
-    for (Group& g : groups_)
+    SpanGroup* group = nullptr;
+    for (SpanGroup& g : groups_)
       if (g.type == type) group = &g;
     if (group == nullptr) {
-      groups_.push_back({type, {}});
+      groups_.push_back({type, {}, {}});
       group = &groups_.back();
     }
     auto& spans = group->spans;
@@ -232,7 +227,7 @@ class Gradients {
   }
 
   torch::Device device_;
-  std::vector<Group> groups_;
+  std::vector<SpanGroup> groups_;
   std::vector<std::pair<const torch::Tensor*, torch::Tensor>> copies_;
 };
 
@@ -277,7 +272,7 @@ struct NormParts {
 NormParts norm_parts(const Gradients& grads, bool inf, float* norm,
                      hipStream_t stream) {
   int64_t n = 0;
-  for (const auto& g : grads.groups()) n += grad_norm_partials(g.spans, g.type);
+  for (const auto& g : grads.groups()) n += g.chunks();
   NormParts out;
   out.buffer = torch::empty(
       {n + 1}, torch::TensorOptions().dtype(at::kDouble).device(grads.device()));
@@ -285,9 +280,11 @@ NormParts norm_parts(const Gradients& grads, bool inf, float* norm,
   uint64_t* sums =
       n == 0 || is_capturing(stream) ? nullptr : sums_of_stream(stream, n);
   int64_t at = 0;
-  for (const auto& g : grads.groups())
-    at += launch_grad_norm_partial(g.spans, g.type, inf, parts, at, n, sums,
-                                   parts + n, norm, stream);
+  for (const auto& g : grads.groups()) {
+    launch_grad_norm_partial(g, inf, parts, at, n, sums, parts + n, norm,
+                             stream);
+    at += g.chunks();
+  }
   out.written = sums != nullptr;
   out.parts = out.written ? parts + n : parts;
   out.n = out.written ? 1 : n;
@@ -333,8 +330,9 @@ torch::Tensor grad_clip_norm(const pybind11::list& list, double max_norm,
   if (!parts.written && grads.groups().empty())
     launch_grad_norm_finish(parts.parts, parts.n, inf, out, stream);
   bool write = !parts.written;  // by the first scaling launch
-  for (const auto& g : grads.groups()) {
-    launch_grad_scale(g.spans, g.type, inf, parts.parts, parts.n, max_norm,
+  const auto& groups = grads.groups();
+  for (auto g = groups.rbegin(); g != groups.rend(); ++g) {
+    launch_grad_scale(*g, inf, parts.parts, parts.n, max_norm,
                       write ? out : nullptr, stream);
     write = false;
   }
@@ -354,7 +352,7 @@ void grad_clip_value(const pybind11::list& list, double clip_value) {
   const c10::DeviceGuard guard(grads.device());
   const auto stream = at::hip::getCurrentHIPStream();
   for (const auto& g : grads.groups())
-    launch_grad_clamp(g.spans, g.type, static_cast<float>(clip_value), stream);
+    launch_grad_clamp(g, static_cast<float>(clip_value), stream);
   C10_HIP_CHECK(hipGetLastError());
   grads.write_copies_back();
   mark_written(tensors);

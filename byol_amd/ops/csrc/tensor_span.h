@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cstdint>
+#include <vector>
 
 // One dense run of elements; `ptr` needs only the element's own alignment.
 struct TensorSpan {
@@ -40,3 +41,26 @@ constexpr int kTableChunks = 1536;
 // every block of the scaling pass (8 KB from L2, and a launch less: 19 us for
 // 22 us on 68 MB below the bound); more are joined in a launch of their own.
 constexpr int64_t kMaxJoinedPartials = kTableChunks + kMaxSpans;
+
+// A table as a kernel argument (under 4 KB).
+struct SpanTable {
+  char* base;  // the lowest address; offsets are in elements
+  uint32_t offset[kMaxSpans];
+  uint32_t len[kMaxSpans];
+  uint16_t first[kMaxSpans + 1];  // a span's first chunk; [count] = all chunks
+  int count;
+  uint32_t chunk;  // elements, a multiple of kLineBytes
+};
+
+// Spans of one type, and their tables.
+struct SpanGroup {
+  SpanType type;
+  std::vector<TensorSpan> spans;
+  std::vector<SpanTable> tables;
+
+  int64_t chunks() const {
+    int64_t n = 0;
+    for (const SpanTable& t : tables) n += t.first[t.count];
+    return n;
+  }
+};
