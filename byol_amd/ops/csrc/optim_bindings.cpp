@@ -21,15 +21,12 @@
 void make_tables(SpanGroup& group);
 void launch_grad_norm_partial(const SpanGroup& group, bool inf,
                               double* partial, int64_t at, int64_t all,
-                              uint64_t* sums, double* joined, float* norm,
+                              uint64_t* sums, double* full, float* rounded,
                               hipStream_t stream);
 void launch_grad_norm_finish(const double* partial, int64_t n, bool inf,
-                             float* norm, hipStream_t stream);
-void launch_grad_norm_join(const double* partial, int64_t n, bool inf,
-                           double* joined, hipStream_t stream);
-void launch_grad_scale(const SpanGroup& group, bool inf,
-                       const double* partial, int64_t n, double bound,
-                       float* norm, hipStream_t stream);
+                             double* full, float* rounded, hipStream_t stream);
+void launch_grad_scale(const SpanGroup& group, const double* norm,
+                       double bound, hipStream_t stream);
 void launch_grad_clamp(const SpanGroup& group, float bound,
                        hipStream_t stream);
 int64_t lamb_chunks(const std::vector<LambTensor>& tensors);
@@ -231,11 +228,6 @@ class Gradients {
   std::vector<std::pair<const torch::Tensor*, torch::Tensor>> copies_;
 };
 
-torch::Tensor one_float(const torch::Device& device) {
-  return torch::empty({},
-                      torch::TensorOptions().dtype(at::kFloat).device(device));
-}
-
 // Places for the sums that a norm's blocks tell each other, "none" in all of
 // them between calls, for the current stream of the current device.  Calls on
 // one stream follow each other, so they share it; calls on other streams have
@@ -260,35 +252,36 @@ bool is_capturing(hipStream_t stream) {
   return status != hipStreamCaptureStatusNone;
 }
 
-// A list's norm on its way: the sums (or largest magnitudes) of n parts, all
-// of which make it up; n is 1 once they are joined, and then `norm` is written.
-struct NormParts {
-  torch::Tensor buffer;  // the parts and, behind them, room for one
-  const double* parts;
-  int64_t n;
-  bool written;
+// The norm of a list, rounded to fp32 and, at the end of its buffer, in full.
+struct Norm {
+  torch::Tensor rounded;
+  torch::Tensor buffer;
+  const double* full;
 };
 
-NormParts norm_parts(const Gradients& grads, bool inf, float* norm,
-                     hipStream_t stream) {
+Norm norm_of(const Gradients& grads, bool inf, hipStream_t stream) {
   int64_t n = 0;
   for (const auto& g : grads.groups()) n += g.chunks();
-  NormParts out;
-  out.buffer = torch::empty(
-      {n + 1}, torch::TensorOptions().dtype(at::kDouble).device(grads.device()));
-  double* parts = out.buffer.data_ptr<double>();
+  const auto options = torch::TensorOptions().device(grads.device());
+  Norm norm;
+  norm.rounded = torch::empty({}, options.dtype(at::kFloat));
+  norm.buffer = torch::empty({n + 1}, options.dtype(at::kDouble));
+  float* rounded = norm.rounded.data_ptr<float>();
+  double* parts = norm.buffer.data_ptr<double>();
+  double* full = parts + n;
+  norm.full = full;
   uint64_t* sums =
       n == 0 || is_capturing(stream) ? nullptr : sums_of_stream(stream, n);
   int64_t at = 0;
   for (const auto& g : grads.groups()) {
-    launch_grad_norm_partial(g, inf, parts, at, n, sums, parts + n, norm,
+    launch_grad_norm_partial(g, inf, parts, at, n, sums, full, rounded,
                              stream);
     at += g.chunks();
   }
-  out.written = sums != nullptr;
-  out.parts = out.written ? parts + n : parts;
-  out.n = out.written ? 1 : n;
-  return out;
+  if (sums == nullptr)
+    launch_grad_norm_finish(parts, n, inf, full, rounded, stream);
+  C10_HIP_CHECK(hipGetLastError());
+  return norm;
 }
 
 torch::Tensor grad_norm(const pybind11::list& list, bool inf) {
@@ -297,14 +290,7 @@ torch::Tensor grad_norm(const pybind11::list& list, bool inf) {
   TORCH_CHECK_VALUE(!tensors.empty(), what, ": no tensors");
   const Gradients grads(tensors, what, false);
   const c10::DeviceGuard guard(grads.device());
-  const auto stream = at::hip::getCurrentHIPStream();
-  auto norm = one_float(grads.device());
-  float* out = norm.data_ptr<float>();
-  const auto parts = norm_parts(grads, inf, out, stream);
-  if (!parts.written)
-    launch_grad_norm_finish(parts.parts, parts.n, inf, out, stream);
-  C10_HIP_CHECK(hipGetLastError());
-  return norm;
+  return norm_of(grads, inf, at::hip::getCurrentHIPStream()).rounded;
 }
 
 torch::Tensor grad_clip_norm(const pybind11::list& list, double max_norm,
@@ -317,29 +303,14 @@ torch::Tensor grad_clip_norm(const pybind11::list& list, double max_norm,
   const Gradients grads(tensors, what, true);
   const c10::DeviceGuard guard(grads.device());
   const auto stream = at::hip::getCurrentHIPStream();
-  auto norm = one_float(grads.device());
-  float* out = norm.data_ptr<float>();
-  auto parts = norm_parts(grads, inf, out, stream);
-  if (!parts.written && (parts.n > kMaxJoinedPartials || parts.n == 0)) {
-    // too many for every block of the scaling pass to join them
-    double* joined = parts.buffer.data_ptr<double>() + parts.n;
-    launch_grad_norm_join(parts.parts, parts.n, inf, joined, stream);
-    parts.parts = joined;
-    parts.n = 1;
-  }
-  if (!parts.written && grads.groups().empty())
-    launch_grad_norm_finish(parts.parts, parts.n, inf, out, stream);
-  bool write = !parts.written;  // by the first scaling launch
+  const Norm norm = norm_of(grads, inf, stream);
   const auto& groups = grads.groups();
-  for (auto g = groups.rbegin(); g != groups.rend(); ++g) {
-    launch_grad_scale(*g, inf, parts.parts, parts.n, max_norm,
-                      write ? out : nullptr, stream);
-    write = false;
-  }
+  for (auto g = groups.rbegin(); g != groups.rend(); ++g)
+    launch_grad_scale(*g, norm.full, max_norm, stream);
   C10_HIP_CHECK(hipGetLastError());
   grads.write_copies_back();
   mark_written(tensors);
-  return norm;
+  return norm.rounded;
 }
 
 void grad_clip_value(const pybind11::list& list, double clip_value) {

@@ -31,16 +31,11 @@ constexpr int64_t kMaxSpanLen = int64_t(1) << 30;
 // chunks, one block for each.  Of 512 to 8192 chunks 1536 measured best or
 // within 2% of it over lists of 46 to 160 MB: fewer leave too few loads in
 // flight (161 MB of fp16: 43 us with 1024, 38 us with 1536), more add sums to
-// join (46 MB of fp32, clipped: 24 us with 1536, 34 us with 8192).  Each
+// join (46 MB of fp32, clipped: 26 us with 1536, 34 us with 8192).  Each
 // further table costs a launch that the one before has to drain for, about
 // 7 us: so a table holds as many spans as an argument of 4 KB can.
 constexpr int kMaxSpans = 352;
 constexpr int kTableChunks = 1536;
-
-// Up to so many partial results of a norm, those of one table, are joined by
-// every block of the scaling pass (8 KB from L2, and a launch less: 19 us for
-// 22 us on 68 MB below the bound); more are joined in a launch of their own.
-constexpr int64_t kMaxJoinedPartials = kTableChunks + kMaxSpans;
 
 // A table as a kernel argument (under 4 KB).
 struct SpanTable {
