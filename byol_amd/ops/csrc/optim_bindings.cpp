@@ -232,19 +232,36 @@ class Gradients {
 // them between calls, for the current stream of the current device.  Calls on
 // one stream follow each other, so they share it; calls on other streams have
 // their own, and graphs, which may be replayed on any stream, have none.
-uint64_t* sums_of_stream(hipStream_t stream, int64_t n) {
-  static std::mutex mutex;
-  static auto* all =  // never freed, so not after the runtime's own end
-      new std::map<std::pair<int, hipStream_t>, torch::Tensor>;
-  const int device = c10::hip::current_device();
-  const std::lock_guard<std::mutex> lock(mutex);
-  auto& sums = (*all)[{device, stream}];
-  if (!sums.defined() || sums.numel() < n)
-    sums = torch::full(
-        {std::max<int64_t>(2 * n, 4096)}, -1,
-        torch::TensorOptions().dtype(at::kLong).device(at::kCUDA, device));
-  return reinterpret_cast<uint64_t*>(sums.data_ptr<int64_t>());
-}
+class StreamSums {
+ public:
+  static uint64_t* get(hipStream_t stream, int64_t n) {
+    const std::lock_guard<std::mutex> lock(mutex());
+    const int device = c10::hip::current_device();
+    auto& sums = all()[{device, stream}];
+    if (!sums.defined() || sums.numel() < n)
+      sums = torch::full(
+          {std::max<int64_t>(2 * n, 4096)}, -1,
+          torch::TensorOptions().dtype(at::kLong).device(at::kCUDA, device));
+    return reinterpret_cast<uint64_t*>(sums.data_ptr<int64_t>());
+  }
+
+  // After a launch that failed: some places may be taken.
+  static void forget(hipStream_t stream) {
+    const std::lock_guard<std::mutex> lock(mutex());
+    all().erase({c10::hip::current_device(), stream});
+  }
+
+ private:
+  using Map = std::map<std::pair<int, hipStream_t>, torch::Tensor>;
+  static std::mutex& mutex() {
+    static std::mutex m;
+    return m;
+  }
+  static Map& all() {
+    static auto* map = new Map;  // never freed, so not after the runtime's end
+    return *map;
+  }
+};
 
 bool is_capturing(hipStream_t stream) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -271,7 +288,7 @@ Norm norm_of(const Gradients& grads, bool inf, hipStream_t stream) {
   double* full = parts + n;
   norm.full = full;
   uint64_t* sums =
-      n == 0 || is_capturing(stream) ? nullptr : sums_of_stream(stream, n);
+      n == 0 || is_capturing(stream) ? nullptr : StreamSums::get(stream, n);
   int64_t at = 0;
   for (const auto& g : grads.groups()) {
     launch_grad_norm_partial(g, inf, parts, at, n, sums, full, rounded,
@@ -280,7 +297,9 @@ Norm norm_of(const Gradients& grads, bool inf, hipStream_t stream) {
   }
   if (sums == nullptr)
     launch_grad_norm_finish(parts, n, inf, full, rounded, stream);
-  C10_HIP_CHECK(hipGetLastError());
+  const hipError_t launched = hipGetLastError();
+  if (launched != hipSuccess && sums != nullptr) StreamSums::forget(stream);
+  C10_HIP_CHECK(launched);
   return norm;
 }
 

@@ -94,6 +94,11 @@ def _reference_step(params, grads, exp_avgs, exp_avg_sqs, decay, step, lr,
         if not p.shape == g.shape == m.shape == v.shape:
             raise ValueError("fused_lamb_step: a gradient or moment has "
                              "another shape than its parameter")
+    devices = {t.device for ts in (params, grads, exp_avgs, exp_avg_sqs)
+               for t in ts}
+    if len(devices) > 1:
+        raise ValueError("fused_lamb_step: expected all tensors on one "
+                         f"device, got {sorted(map(str, devices))}")
     check_writable([*params, *exp_avgs, *exp_avg_sqs], "fused_lamb_step")
     factor = 1.0
     if grad_norm is not None:

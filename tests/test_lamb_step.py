@@ -373,6 +373,19 @@ def test_optimizer_mixes_fused_and_single_parameters():
 
 
 @pytest.mark.gpu
+def test_devices_do_not_mix():
+    _, lists = make([64, 8], "cpu")
+    before = [t.clone() for ts in lists for t in ts]
+    for k in range(4):
+        mixed = [[t.cuda() if i == k else t for t in ts]
+                 for i, ts in enumerate(lists)]
+        with pytest.raises(ValueError, match="expected"):
+            ops.fused_lamb_step(*mixed, step=1, lr=0.1)
+    assert all(torch.equal(t, b) for t, b in
+               zip((t for ts in lists for t in ts), before))
+
+
+@pytest.mark.gpu
 def test_step_refuses_capture():
     _, lists = make([64], "cuda")
     before = lists[0][0].clone()
