@@ -198,6 +198,9 @@ struct NormEnd {
 
 constexpr uint64_t kJoinTicks = 1000000000;  // of 10 ns
 
+// Leaves what it reads in the caches, though streaming past them is faster by
+// itself (148 MB: 26 us for 29): the step that follows reads the gradients
+// again, and LAMB with its clipping takes 220 us so and 239 otherwise.
 template <typename T, typename Reduce>
 __global__ __launch_bounds__(kSpanBlock) void grad_norm_partial_kernel(
     const SpanTable table, double* __restrict__ partial, int at,
