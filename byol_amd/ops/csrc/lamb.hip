@@ -19,10 +19,10 @@
 // which reads p, m and v again and computes the same values.
 //
 // Bound by memory: 37 M parameters (ResNet-50 with its heads) take 202 us in
-// one launch, 5.1 TB/s, 76 M (ResNet-200) 373 us, 5.7 TB/s; in two passes the
-// first took 250 us.  All of p, m and v is read and written past the caches,
-// where nothing is left of it until the next step (262 us for 250 without that,
-// at 8192 elements a block).
+// one launch, 5.1 TB/s, 76 M (ResNet-200) 373 us, 5.7 TB/s.  Two passes over all
+// tensors took 257 us for the first.  All of p, m and v is read and written past
+// the caches, where nothing is left of it until the next step (262 us for 250
+// without that, at 8192 elements a block).
 #include "multi_tensor.h"
 
 #include <algorithm>
@@ -131,7 +131,7 @@ __device__ __forceinline__ float lamb_factor(double pp, double uu, float lr) {
 
 // Adds up the sums of chunks [c0, c1) over the block, in a fixed order.  Each
 // sum is valid by itself (it is not kNoSum), so no other order between blocks
-// is needed.  With `wait`, sums that are missing are waited for until the time
+// is needed.  With kWait, sums that are missing are waited for until the time
 // is up; returns whether all were there, the same in all threads.
 template <bool kWait>
 __device__ __forceinline__ bool join_sums(const uint64_t* sums, int c0, int c1,
@@ -207,9 +207,10 @@ struct LambChunk {
   }
 };
 
+constexpr int kWavesPerSimd = kBlocksPerCu * kLambBlock / (4 * WAVE_SIZE);
+
 template <typename G>
-__global__ __launch_bounds__(
-    kLambBlock, kBlocksPerCu * kLambBlock / (4 * WAVE_SIZE)) void lamb_step_kernel(
+__global__ __launch_bounds__(kLambBlock, kWavesPerSimd) void lamb_step_kernel(
     const LambList list, LambRates r, const float* __restrict__ norm,
     double max_norm, uint64_t wait_ticks) {
   __shared__ Pack4 kept[kLdsPacks * kLambBlock];

@@ -3,7 +3,7 @@
 ``N = sqrt(sum_t ||g_t||^2)`` (or the largest magnitude), then
 ``g <- min(1, max_norm / (N + 1e-6)) * g``; by value, ``g`` is bounded to
 ``[-clip_value, clip_value]``.  The reference clips by value before its
-optimizer step (``/root/reference/main.py:618-624``).
+optimizer step (its ``main.py:618-624``).
 
 On GPU a list of any length is a few launches of the kernels in
 ``csrc/gradclip.hip`` and never waits for the host, so the calls can be

@@ -6,11 +6,11 @@ With ``g' = c g`` (``c`` the global-norm clipping factor, or 1)::
     u = (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps) + wd p
     p = p - lr r u,   r = ||p|| / ||u|| of the tensor (1 if either is 0)
 
-The reference takes Apex's fused optimizer for this
-(``/root/reference/main.py:324-326``).  On GPU a step is two passes of the
-kernels in ``csrc/lamb.hip`` over all tensors together and never waits for the
-host; clipping costs one more reading of the gradients, which stay as they
-are.  Elsewhere the same step runs tensor by tensor in torch operations.
+The reference takes an external fused optimizer for this (its
+``main.py:324-326``).  On GPU a step is one pass of the kernels in
+``csrc/lamb.hip`` over all tensors together and never waits for the host;
+clipping costs one more reading of the gradients, which stay as they are.
+Elsewhere the same step runs tensor by tensor in torch operations.
 """
 
 from typing import Optional, Sequence, Tuple, Union

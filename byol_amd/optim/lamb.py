@@ -1,13 +1,12 @@
-"""LAMB optimizer (replacement for the reference's Apex FusedLAMB,
-``/root/reference/main.py:324-326``): the LAMB update (You et al.,
-arXiv:1904.00962) — Adam-style moments, then a per-layer trust ratio
-``||p|| / ||update||`` scales the step.
+"""LAMB optimizer (the reference takes one from another package, its
+``main.py:324-326``): the LAMB update (You et al., arXiv:1904.00962) —
+Adam-style moments, then a per-layer trust ratio ``||p|| / ||update||`` scales
+the step.
 
 fp32 parameters on a GPU take the fused step (``byol_amd/ops/lamb_step.py``):
-all tensors in two passes, without a host wait.  Other parameters are updated
-one by one in torch operations.  ``max_grad_norm`` clips the global norm of
-all gradients inside the step, as Apex's optimizer does; the gradients
-themselves are left as they are.
+all tensors together, without a host wait.  Other parameters are updated one by
+one in torch operations.  ``max_grad_norm`` clips the global norm of all
+gradients inside the step; the gradients themselves are left as they are.
 """
 
 import torch

@@ -238,6 +238,34 @@ def test_one_tensor_is_a_list_of_it(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_thousands_of_tensors_then_few(device):
+    _, many = make([1 + i % 5 for i in range(9000)], torch.float32, device,
+                   gap=1)
+    few = [torch.tensor(3.0, device=device), torch.full((2, 2), 2.0,
+                                                        device=device)]
+    for _ in range(2):
+        check_norm(ops.global_grad_norm(few), 5.0)
+        check_norm(ops.global_grad_norm(many), exact_norm(many, 2.0))
+    before = [g.clone() for g in many]
+    want = exact_norm(many, 2.0)
+    check_norm(ops.clip_grads_by_norm_(many, 1.0), want)
+    for g, b in zip(many[::97], before[::97]):
+        check_scaled(g, b, want, 1.0)
+    check_norm(ops.clip_grads_by_norm_(few, 1.0), 5.0)
+    assert few[0].dim() == 0 and abs(few[0].item() - 0.6) < 1e-6
+
+
+@pytest.mark.gpu
+def test_inside_inference_mode():
+    with torch.inference_mode():
+        g = torch.full((100,), 2.0, device="cuda")
+        check_norm(ops.clip_grads_by_norm_([g], 5.0), 20.0)
+        check_scaled(g, torch.full((100,), 2.0), 20.0, 5.0)
+        ops.clip_grads_by_value_([g], 0.25)
+        assert (g == 0.25).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_refusals(device):
     g = torch.ones(64, device=device)
     calls = [lambda t: ops.clip_grads_by_norm_(t, 0.1),

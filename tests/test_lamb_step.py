@@ -414,6 +414,15 @@ def test_two_streams():
 
 
 @pytest.mark.gpu
+def test_thousands_of_tensors():
+    _, lists = make([1 + i % 7 for i in range(3000)], "cuda", gap=1)
+    before = [[t.clone() for t in ts] for ts in lists]
+    ops.fused_lamb_step(*lists, step=2, lr=0.1)
+    some = [[ts[i] for i in range(0, 3000, 59)] for ts in (*lists, *before)]
+    check(some[:4], some[4:], 2, 0.1, 1e-6, [0.0] * len(some[0]))
+
+
+@pytest.mark.gpu
 def test_gradients_far_apart():
     """More than 2^32 elements between the gradients of two parameters."""
     sizes = [2000, 40_000, 7]
