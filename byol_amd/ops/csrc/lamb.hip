@@ -56,7 +56,7 @@ struct LambList {
   int chunks;      // of all of them
   int max_wait;    // the most chunks of a tensor that wait for each other
   uint64_t* sums;  // 2 for each chunk: of p^2, of u^2, as bits of doubles
-  double* totals;  // 2 for each tensor of too many chunks to wait for
+  double* totals;  // 2 for each tensor of more than kMaxJoined chunks
   int* done;       // for each chunk: p is updated
   int* undone;     // whether any chunk is left to the second pass
 };
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(kLambBlock, kWavesPerSimd) void lamb_step_kernel(
       store_sum(list.sums + 2 * c, pp);
       store_sum(list.sums + 2 * c + 1, uu);
     }
-    const bool waits = c1 - c0 <= list.max_wait && wait_ticks > 0;
+    const bool waits = c1 - c <= list.max_wait && wait_ticks > 0;
     if (!waits || !join_sums<true>(list.sums, c0, c1, wait_ticks, scratch,
                                    &pp, &uu)) {
       if (threadIdx.x == 0)
@@ -321,14 +321,16 @@ __global__ __launch_bounds__(kLambBlock, kWavesPerSimd) void lamb_step_kernel(
   if (threadIdx.x == 0) list.done[c] = 1;
 }
 
-// The sums of tensors that have too many chunks for every block of the second
-// pass to join them.
+// A tensor of more chunks than this has its sums joined once before the second
+// pass, where otherwise every block of it joins them (up to 32 KB).
+constexpr int kMaxJoined = 2048;
+
 __global__ __launch_bounds__(kLambBlock) void lamb_totals_kernel(
     const LambList list) {
   __shared__ double scratch[kLambBlock / WAVE_SIZE];
   const int s = blockIdx.x;
   const int c0 = list.first[s], c1 = list.first[s + 1];
-  if (c1 - c0 <= list.max_wait) return;
+  if (c1 - c0 <= kMaxJoined) return;
   double pp, uu;
   join_sums<false>(list.sums, c0, c1, 0, scratch, &pp, &uu);
   if (threadIdx.x != 0) return;
@@ -349,13 +351,14 @@ __global__ __launch_bounds__(kLambBlock) void lamb_rest_kernel(
     float* p = chunk.p;
     const float *m = chunk.m, *v = chunk.v;
     double pp, uu;
-    if (c1 - c0 > list.max_wait) {
+    if (c1 - c0 > kMaxJoined) {
       pp = list.totals[2 * s];
       uu = list.totals[2 * s + 1];
     } else {
       join_sums<false>(list.sums, c0, c1, 0, scratch, &pp, &uu);
     }
     const float step = lamb_factor(pp, uu, r.lr);
+    #pragma unroll 2
     for (uint32_t i = threadIdx.x; i < chunk.last; i += kLambBlock) {
       if (i < chunk.first) continue;
       Pack4* at = reinterpret_cast<Pack4*>(p) + i;
@@ -376,8 +379,12 @@ __global__ __launch_bounds__(kLambBlock) void lamb_rest_kernel(
   }
 }
 
-// Four of five blocks that run at a time: a tensor of more chunks could not
-// count on all of them being there.
+// One block for each CU.  Two have room, but where blocks that wait and blocks
+// that do not share the chip, a CU's second place sometimes stays empty while a
+// block that is waited for has not started.  On a list of 28 M elements, 20 M
+// of them in one tensor, a step in two ran into the time limit with 409 of 512
+// blocks waiting, one in a hundred with 320, none with 256; it takes 195 us so,
+// and 230 us if none wait.
 int max_wait_chunks() {
   static int cus[64] = {};
   int device = 0;
@@ -386,7 +393,7 @@ int max_wait_chunks() {
   if (cus[device] == 0)
     (void)hipDeviceGetAttribute(&cus[device],
                                 hipDeviceAttributeMultiprocessorCount, device);
-  return kBlocksPerCu * cus[device] * 4 / 5;
+  return cus[device];
 }
 
 int64_t chunks_of(const LambTensor& t) {
@@ -496,7 +503,7 @@ void launch_lamb_step(std::vector<LambTensor>& tensors, int64_t chunks,
       piece.decay[i] = t.decay;
       const int own = static_cast<int>(chunks_of(t));
       first += own;
-      long_tensors = long_tensors || own > list.max_wait;
+      long_tensors = long_tensors || own > kMaxJoined;
     }
     const int blocks = at == 0 ? grid_1d(n, kLambBlock, 64) : 1;
     hipLaunchKernelGGL(lamb_list_kernel, dim3(blocks), block, 0, stream, piece,
@@ -511,6 +518,6 @@ void launch_lamb_step(std::vector<LambTensor>& tensors, int64_t chunks,
     hipLaunchKernelGGL(lamb_totals_kernel, dim3(count), block, 0, stream,
                        list);
   if (n > count)  // some tensor has more than one chunk
-    hipLaunchKernelGGL(lamb_rest_kernel, dim3(std::min(n, 512)), block, 0,
+    hipLaunchKernelGGL(lamb_rest_kernel, dim3(std::min(n, 1024)), block, 0,
                        stream, list, r);
 }

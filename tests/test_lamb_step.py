@@ -132,7 +132,7 @@ def test_step(device, dtype, step, clip, sizes):
 @pytest.mark.gpu
 @pytest.mark.parametrize("sizes", [[5_000_001, 3, 700_000],
                                    [70_000] * 100,
-                                   [10_000_003, 8192, 8193, 9_000_000]])
+                                   [70_000_003, 32768, 32769, 14_000_000]])
 def test_large_lists(sizes):
     _, lists = make(sizes, "cuda", gap=1)
     before = [[t.clone() for t in ts] for ts in lists]
@@ -173,7 +173,7 @@ def test_every_alignment(wait_ticks):
 def test_second_pass_gives_the_same_bits(dtype, wait_ticks):
     """Blocks that do not wait for the rest of their tensor, or give up, leave
     it to a pass that computes the same."""
-    sizes = [3_000_001, 8192, 8193, 20_000, 5, 100_000] * 3
+    sizes = [3_000_001, 32768, 32769, 20_000, 5, 100_000] * 3 + [15_000_000]
     results = []
     for ticks in (20000, wait_ticks):
         _, lists = make(sizes, "cuda", dtype, gap=1)
