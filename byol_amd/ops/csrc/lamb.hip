@@ -14,9 +14,10 @@
 //
 // The wait needs the other blocks to run at the same time, which nothing
 // guarantees: a tensor may have more chunks than fit the chip, and other work
-// may hold it.  So tensors of too many chunks do not wait, a wait ends after a
-// set time, and a block that gave up leaves its part of p to a second pass,
-// which reads p, m and v again and computes the same values.
+// may hold it.  So only the last chunks of a tensor wait, one for each CU (8.4 M
+// elements); a wait ends after a set time; and a block that does not wait, or
+// gave up, leaves its part of p to a second pass, which reads p, m and v again
+// and computes the same values.
 //
 // Bound by memory: 37 M parameters (ResNet-50 with its heads) take 202 us in
 // one launch, 5.1 TB/s, 76 M (ResNet-200) 373 us, 5.7 TB/s.  Two passes over all
@@ -37,11 +38,23 @@ namespace {
 // tensor of 8.4 M) takes 250 us with 8192 elements in each of 5 blocks of 256
 // threads, 232 us with 16384 in each of 3, and 229 us so; ResNet-200's with its
 // clipping 519, 489 and 462 us (in the order of the modules, see below).
+//
+// Short lists would leave CUs idle at that size: their blocks take 8192, all in
+// registers.  2 M elements take 22 us so and 33 us otherwise, 4.1 M 32 and 36,
+// 5 M (where not all blocks of a tensor may wait any more) 48 and 38.
 constexpr int kLambBlock = 512;
-constexpr int kPacks = 16;    // packs of 4 elements of one thread
-constexpr int kLdsPacks = 9;  // of them with p in LDS, the others in registers
-constexpr int kLambChunk = kLambBlock * 4 * kPacks;
-constexpr int kBlocksPerCu = 2;
+constexpr int kLongPacks = 16;  // packs of 4 elements of one thread
+constexpr int kShortPacks = 4;
+constexpr int64_t kShortList = int64_t(1) << 22;  // elements
+
+// Of a thread's packs, those with p in LDS, the others in registers.
+constexpr int lds_packs(int packs) { return packs == kLongPacks ? 9 : 0; }
+
+// Blocks that share a CU: by LDS and 128 registers, or by 80 registers.
+constexpr int blocks_per_cu(int packs) { return packs == kLongPacks ? 2 : 3; }
+
+// Elements of a block.
+constexpr int chunk_of(int packs) { return kLambBlock * 4 * packs; }
 
 // The tensors of a step in device memory, and what its blocks tell each other.
 struct LambList {
@@ -54,6 +67,7 @@ struct LambList {
   float* decay;
   int count;       // tensors
   int chunks;      // of all of them
+  uint32_t chunk;  // elements
   int max_wait;    // the most chunks of a tensor that wait for each other
   uint64_t* sums;  // 2 for each chunk: of p^2, of u^2, as bits of doubles
   double* totals;  // 2 for each tensor of more than kMaxJoined chunks
@@ -180,10 +194,10 @@ struct LambChunk {
     c0 = list.first[s];
     c1 = list.first[s + 1];
     const uint32_t before = line_offset(list.p[s]);
-    const uint32_t at = uint32_t(c - c0) * kLambChunk;
+    const uint32_t at = uint32_t(c - c0) * list.chunk;
     const uint32_t stop = before + list.len[s] - at;
     begin = at == 0 ? before : 0;
-    end = stop < kLambChunk ? stop : kLambChunk;
+    end = stop < list.chunk ? stop : list.chunk;
     const int64_t move = int64_t(at) - before;
     p = list.p[s] + move;
     m = list.m[s] + move;
@@ -199,21 +213,25 @@ struct LambChunk {
     const uint32_t e = t < 4 ? begin + t : tail + t - 4;
     edge = t < 8 && e < (t < 4 ? head : end) ? e : kNone;
   }
-  __device__ __forceinline__ bool whole() const {
-    return begin == 0 && end == kLambChunk;
+  __device__ __forceinline__ bool whole(uint32_t size) const {
+    return begin == 0 && end == size;
   }
   __device__ __forceinline__ bool has(uint32_t pack) const {
     return pack >= first && pack < last;
   }
 };
 
-constexpr int kWavesPerSimd = kBlocksPerCu * kLambBlock / (4 * WAVE_SIZE);
+constexpr int waves_per_simd(int packs) {
+  return blocks_per_cu(packs) * kLambBlock / (4 * WAVE_SIZE);
+}
 
-template <typename G>
-__global__ __launch_bounds__(kLambBlock, kWavesPerSimd) void lamb_step_kernel(
+template <typename G, int kPacks>
+__global__
+__launch_bounds__(kLambBlock, waves_per_simd(kPacks)) void lamb_step_kernel(
     const LambList list, LambRates r, const float* __restrict__ norm,
     double max_norm, uint64_t wait_ticks) {
-  __shared__ Pack4 kept[kLdsPacks * kLambBlock];
+  constexpr int kLdsPacks = lds_packs(kPacks);
+  __shared__ Pack4 kept[kLdsPacks > 0 ? kLdsPacks * kLambBlock : 1];
   __shared__ float2 edge[8];  // p and u of single elements
   __shared__ double scratch[kLambBlock / WAVE_SIZE];
   typedef G PackG __attribute__((ext_vector_type(4), aligned(sizeof(G))));
@@ -263,7 +281,7 @@ __global__ __launch_bounds__(kLambBlock, kWavesPerSimd) void lamb_step_kernel(
     else
       last[k - kLdsPacks] = pv;
   };
-  if (chunk.whole()) {
+  if (chunk.whole(chunk_of(kPacks))) {
     #pragma unroll
     for (int k = 0; k < kPacks; ++k) pack(k);
   } else {
@@ -306,7 +324,7 @@ __global__ __launch_bounds__(kLambBlock, kWavesPerSimd) void lamb_step_kernel(
     __builtin_nontemporal_store(
         pv, reinterpret_cast<Pack4*>(p) + threadIdx.x + k * kLambBlock);
   };
-  if (chunk.whole()) {
+  if (chunk.whole(chunk_of(kPacks))) {
     #pragma unroll
     for (int k = 0; k < kPacks; ++k) update(k);
   } else {
@@ -379,13 +397,13 @@ __global__ __launch_bounds__(kLambBlock) void lamb_rest_kernel(
   }
 }
 
-// One block for each CU.  Two have room, but where blocks that wait and blocks
-// that do not share the chip, a CU's second place sometimes stays empty while a
+// One block less for each CU than have room.  Where blocks that wait and blocks
+// that do not share the chip, a CU's last place sometimes stays empty while a
 // block that is waited for has not started.  On a list of 28 M elements, 20 M
 // of them in one tensor, a step in two ran into the time limit with 409 of 512
 // blocks waiting, one in a hundred with 320, none with 256; it takes 195 us so,
 // and 230 us if none wait.
-int max_wait_chunks() {
+int max_wait_chunks(int packs) {
   static int cus[64] = {};
   int device = 0;
   if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64)
@@ -393,11 +411,11 @@ int max_wait_chunks() {
   if (cus[device] == 0)
     (void)hipDeviceGetAttribute(&cus[device],
                                 hipDeviceAttributeMultiprocessorCount, device);
-  return cus[device];
+  return (blocks_per_cu(packs) - 1) * cus[device];
 }
 
-int64_t chunks_of(const LambTensor& t) {
-  return (line_offset(t.p) + t.len + kLambChunk - 1) / kLambChunk;
+int64_t chunks_of(const LambTensor& t, int packs) {
+  return (line_offset(t.p) + t.len + chunk_of(packs) - 1) / chunk_of(packs);
 }
 
 // The list's arrays one after the other in `bytes` of workspace.
@@ -411,6 +429,7 @@ LambList lay_out(char* at, int count, int chunks, size_t* bytes) {
   LambList list;
   list.count = count;
   list.chunks = chunks;
+  list.chunk = 0;
   list.max_wait = 0;
   list.p = reinterpret_cast<float**>(take(count * sizeof(float*)));
   list.g = reinterpret_cast<const void**>(take(count * sizeof(void*)));
@@ -429,10 +448,12 @@ LambList lay_out(char* at, int count, int chunks, size_t* bytes) {
 
 }  // namespace
 
-int64_t lamb_chunks(const std::vector<LambTensor>& tensors) {
-  int64_t n = 0;
-  for (const LambTensor& t : tensors) n += chunks_of(t);
-  return n;
+LambPlan lamb_plan(const std::vector<LambTensor>& tensors) {
+  int64_t total = 0;
+  for (const LambTensor& t : tensors) total += t.len;
+  LambPlan plan = {total <= kShortList ? kShortPacks : kLongPacks, 0};
+  for (const LambTensor& t : tensors) plan.chunks += chunks_of(t, plan.packs);
+  return plan;
 }
 
 int64_t lamb_workspace_bytes(int64_t count, int64_t chunks) {
@@ -441,7 +462,7 @@ int64_t lamb_workspace_bytes(int64_t count, int64_t chunks) {
   return static_cast<int64_t>(bytes);
 }
 
-void launch_lamb_step(std::vector<LambTensor>& tensors, int64_t chunks,
+void launch_lamb_step(std::vector<LambTensor>& tensors, const LambPlan& plan,
                       SpanType type, double lr, double beta1, double beta2,
                       double eps, int64_t step, const float* norm,
                       double max_norm, int64_t wait_ticks, void* workspace,
@@ -463,10 +484,11 @@ void launch_lamb_step(std::vector<LambTensor>& tensors, int64_t chunks,
   r.eps = static_cast<float>(eps);
   r.lr = static_cast<float>(lr);
   const int count = static_cast<int>(tensors.size());
-  const int n = static_cast<int>(chunks);
+  const int n = static_cast<int>(plan.chunks);
   size_t bytes;
   LambList list = lay_out(static_cast<char*>(workspace), count, n, &bytes);
-  list.max_wait = max_wait_chunks();
+  list.chunk = chunk_of(plan.packs);
+  list.max_wait = max_wait_chunks(plan.packs);
   const dim3 block(kLambBlock);
   bool long_tensors = false;
   int first = 0;
@@ -501,7 +523,7 @@ void launch_lamb_step(std::vector<LambTensor>& tensors, int64_t chunks,
       piece.len[i] = static_cast<uint32_t>(t.len);
       piece.first[i] = first;
       piece.decay[i] = t.decay;
-      const int own = static_cast<int>(chunks_of(t));
+      const int own = static_cast<int>(chunks_of(t, plan.packs));
       first += own;
       long_tensors = long_tensors || own > kMaxJoined;
     }
@@ -510,9 +532,15 @@ void launch_lamb_step(std::vector<LambTensor>& tensors, int64_t chunks,
                        list);
   }
   with_element_type(type, [&](auto value) {
-    hipLaunchKernelGGL((lamb_step_kernel<decltype(value)>), dim3(n), block, 0,
-                       stream, list, r, norm, max_norm,
-                       static_cast<uint64_t>(wait_ticks));
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(n), block, 0, stream, list, r, norm,
+                         max_norm, static_cast<uint64_t>(wait_ticks));
+    };
+    using G = decltype(value);
+    if (plan.packs == kShortPacks)
+      launch(lamb_step_kernel<G, kShortPacks>);
+    else
+      launch(lamb_step_kernel<G, kLongPacks>);
   });
   if (long_tensors)
     hipLaunchKernelGGL(lamb_totals_kernel, dim3(count), block, 0, stream,

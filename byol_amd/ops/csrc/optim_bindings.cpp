@@ -29,9 +29,9 @@ void launch_grad_scale(const SpanGroup& group, const double* norm,
                        double bound, hipStream_t stream);
 void launch_grad_clamp(const SpanGroup& group, float bound,
                        hipStream_t stream);
-int64_t lamb_chunks(const std::vector<LambTensor>& tensors);
+LambPlan lamb_plan(const std::vector<LambTensor>& tensors);
 int64_t lamb_workspace_bytes(int64_t count, int64_t chunks);
-void launch_lamb_step(std::vector<LambTensor>& tensors, int64_t chunks,
+void launch_lamb_step(std::vector<LambTensor>& tensors, const LambPlan& plan,
                       SpanType type, double lr, double beta1, double beta2,
                       double eps, int64_t step, const float* norm,
                       double max_norm, int64_t wait_ticks, void* workspace,
@@ -460,12 +460,13 @@ void lamb_step(const pybind11::list& param_list,
                     static_cast<float>(decay[i])});
   }
   if (list.empty()) return;
-  const int64_t chunks = lamb_chunks(list);
-  TORCH_CHECK_VALUE(chunks < (int64_t(1) << 30), what, ": too many elements");
+  const LambPlan plan = lamb_plan(list);
+  TORCH_CHECK_VALUE(plan.chunks < (int64_t(1) << 30), what, ": too many elements");
   auto workspace = torch::empty(
-      {lamb_workspace_bytes(static_cast<int64_t>(list.size()), chunks)},
+      {lamb_workspace_bytes(static_cast<int64_t>(list.size()),
+                            plan.chunks)},
       torch::TensorOptions().dtype(at::kByte).device(device));
-  launch_lamb_step(list, chunks, grad_type, lr, beta1, beta2, eps, step,
+  launch_lamb_step(list, plan, grad_type, lr, beta1, beta2, eps, step,
                    norm_ptr, max_norm, wait_ticks, workspace.data_ptr(),
                    at::hip::getCurrentHIPStream());
   C10_HIP_CHECK(hipGetLastError());

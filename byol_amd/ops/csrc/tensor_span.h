@@ -20,6 +20,12 @@ struct LambTensor {
   float decay;
 };
 
+// How a LAMB step cuts its tensors: 2048 elements times `packs` for a block.
+struct LambPlan {
+  int packs;
+  int64_t chunks;
+};
+
 // Element types of a span, as the bindings name them.
 enum class SpanType { kF32, kBF16, kF16 };
 

@@ -102,7 +102,7 @@ LISTS = {
     "one bias": [257],
     "no values among some": [0, 5, 0, 64],
     "around a pack": [3, 4, 5, 7, 8, 9],
-    "around a block's share": [4095, 4096, 4097, 8191],
+    "around a block's share": [8191, 8192, 8193, 16383, 24577],
     "more tensors than a table": [1 + (i * 37) % 300 for i in range(200)],
 }
 
@@ -149,8 +149,9 @@ def test_large_lists(sizes):
 @pytest.mark.parametrize("wait_ticks", [0, 20000])
 def test_every_alignment(wait_ticks):
     """Each place in a cache line, lengths around it and around a block's
-    share; parameters aligned unlike their moments."""
-    for n in (1, 2, 3, 4, 5, 31, 32, 33, 32767, 32768, 32769, 70_000):
+    share in short and in long lists; parameters aligned unlike moments."""
+    for n in (1, 2, 3, 4, 5, 31, 32, 33, 8191, 8192, 8193, 70_000, 163_840,
+              196_607):
         sizes = [n + i for i in range(9)] * 3
         arenas, lists = make(sizes, "cuda", gap=3)
         moved = [torch.empty(sum(sizes) + 40, device="cuda") for _ in "gm"]
@@ -170,10 +171,12 @@ def test_every_alignment(wait_ticks):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("wait_ticks", [0, 1, 1000])
-def test_second_pass_gives_the_same_bits(dtype, wait_ticks):
+@pytest.mark.parametrize("sizes", [
+    [3_000_001, 32768, 32769, 20_000, 5, 100_000] * 3 + [15_000_000],
+    [400_001, 8192, 8193, 5, 100_000] * 3])
+def test_second_pass_gives_the_same_bits(dtype, wait_ticks, sizes):
     """Blocks that do not wait for the rest of their tensor, or give up, leave
     it to a pass that computes the same."""
-    sizes = [3_000_001, 32768, 32769, 20_000, 5, 100_000] * 3 + [15_000_000]
     results = []
     for ticks in (20000, wait_ticks):
         _, lists = make(sizes, "cuda", dtype, gap=1)
