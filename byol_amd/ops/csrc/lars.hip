@@ -1,5 +1,5 @@
 // Fused multi-tensor LARS + SGD-momentum step over the flat parameter space.
-// Three launches replace the reference's ~6 ATen kernels x ~160 tensors
+// Three launches, behind one that clears the sums, replace the reference's ~6 ATen kernels x ~160 tensors
 // (/root/reference/optimizers/lars.py:84-127 + torch SGD):
 //   1. lars_norms_kernel  — per-segment sum(p^2) and sum((g+wd*p)^2),
 //      block-per-chunk (chunk table precomputed host-side) with atomic
@@ -9,6 +9,12 @@
 //   3. lars_update_kernel — g_eff = (g + wd*p) * alr[seg];
 //      m = momentum*m + g_eff (first step: m = g_eff); p -= lr*m.
 #include "common.h"
+
+// A kernel, as memory-set nodes of a captured step are not dependable on replay.
+__global__ void lars_clear_kernel(float* __restrict__ norm_acc, int n) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n) norm_acc[i] = 0.f;
+}
 
 __global__ void lars_norms_kernel(const float* __restrict__ p,
                                   const float* __restrict__ g,
@@ -105,7 +111,8 @@ void launch_lars_momentum_step(float* p, const float* g, float* m,
                                const float* lr_dev,
                                float momentum, int m_init,
                                hipStream_t stream) {
-  (void)hipMemsetAsync(norm_acc, 0, sizeof(float) * 2 * nseg, stream);
+  hipLaunchKernelGGL(lars_clear_kernel, dim3((2 * nseg + 255) / 256),
+                     dim3(256), 0, stream, norm_acc, 2 * nseg);
   hipLaunchKernelGGL(lars_norms_kernel, dim3(nchunks), dim3(256), 0, stream,
                      p, g, norm_acc, seg_off, seg_len, seg_wd, chunk_seg,
                      chunk_base, chunk, nchunks);

@@ -499,3 +499,49 @@ def test_refuses_to_wait_while_captured():
     graph.replay()
     torch.cuda.synchronize()
     check_scaled(p.grad, torch.ones(8), math.sqrt(8), 1.0)
+
+
+@pytest.mark.gpu
+def test_captured_with_the_lars_step():
+    """Clipping and the fused LARS step in one graph.  Every tensor is below
+    the step's chunk of 65536, so that one block sums it and the bits are the
+    eager ones on every replay."""
+    from byol_amd import layers
+    from byol_amd.models.byol import FlatParamSpace
+    from byol_amd.optim.lars import LARS
+
+    def build():
+        torch.manual_seed(3)
+        net = torch.nn.Sequential(*(torch.nn.Linear(61, 61)
+                                    for _ in range(5))).cuda()
+        space = FlatParamSpace(net)
+        space.flatten()
+        opt = LARS(torch.optim.SGD(layers.add_weight_decay(net, 1e-4), lr=0.05,
+                                   momentum=0.9))
+        opt.attach_flat_space(space)
+
+        def step():
+            norm = clip_grad_norm_(net.parameters(), 0.5)
+            opt.step()
+            return norm
+        return space, opt, step
+
+    (want, _, eager), (got, opt, captured) = build(), build()
+    values = [torch.randn_like(want.flat_grads) * 10.0 ** (turn - 2)
+              for turn in range(5)]
+    for space, step in ((want, eager), (got, captured)):
+        space.flat_grads.copy_(values[0])
+        step()  # makes the momentum
+    opt._fused.lr_dev.fill_(0.05)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = captured()
+    for value in values[1:]:
+        got.flat_grads.copy_(value)
+        graph.replay()
+        want.flat_grads.copy_(value)
+        expect = eager()
+        torch.cuda.synchronize()
+        assert torch.equal(norm, expect)
+        assert torch.equal(got.flat_params, want.flat_params)
