@@ -152,23 +152,28 @@ struct LoadPartials {
   }
 };
 
-// From blocks that may still run: waits for each sum and takes it out.
+// From blocks that may still run: waits for each sum.  `missing` becomes the
+// lowest place that has none when the time is up; the place is looked at once
+// more then, as the block itself may have stood still.
 template <int kThreads>
-struct TakePartials {
-  uint64_t* sums;
+struct AwaitPartials {
+  const uint64_t* sums;
   uint64_t until;
+  int* missing;
   __device__ __forceinline__ void operator()(int i, double* v, int n) const {
     uint64_t bits[4];
     #pragma unroll
     for (int k = 0; k < n; ++k) bits[k] = load_sum(sums + i + k * kThreads);
     #pragma unroll
     for (int k = 0; k < n; ++k) {
-      uint64_t* at = sums + i + k * kThreads;
-      while (bits[k] == kNoSum && wall_clock64() < until) {
+      const int place = i + k * kThreads;
+      bool late = false;
+      while (bits[k] == kNoSum && !late) {
+        late = wall_clock64() >= until;
         __builtin_amdgcn_s_sleep(1);
-        bits[k] = load_sum(at);
+        bits[k] = load_sum(sums + place);
       }
-      *at = kNoSum;
+      if (bits[k] == kNoSum && place < *missing) *missing = place;
       v[k] = sum_value(bits[k]);
     }
   }
@@ -188,15 +193,51 @@ struct NormOut {
 // How partial results become a norm.  With `sums`, the last block of the
 // call's last launch joins them as they come in: a launch less, 3 us for the
 // host and 4 us for the GPU.  It waits only for blocks that wait for nothing
-// themselves.  The time limit is for a device that has failed; the norm is NaN
-// then.
+// themselves, and only for a time: it then computes what is missing itself,
+// with the same bits.
+//
+// A block that was late writes its sum all the same, after it was read for the
+// last time.  So calls take two sets of places in turn, and each call clears
+// the set of the call before it, whose blocks have all ended.
 struct NormEnd {
-  uint64_t* sums;  // kNoSum in all before and after the call; or null
-  int all;         // blocks of all launches of the call
+  uint64_t* sums;   // this call's places, kNoSum in all before it; or null
+  uint64_t* clear;  // the places of the call before, and how many it used
+  int cleared;
+  int all;          // blocks of all launches of the call
+  uint64_t wait_ticks;  // of 10 ns
   NormOut out;
 };
 
-constexpr uint64_t kJoinTicks = 1000000000;  // of 10 ns
+// A block's share of a norm: four packs of a thread at a time, or one (kWide
+// false), in the same order and so with the same bits.
+template <typename T, typename Reduce, bool kWide>
+__device__ __forceinline__ double chunk_sum(const Chunk<const T>& chunk,
+                                            double* scratch) {
+  using V = typename Pack<T>::type;
+  constexpr int L = Pack<T>::kLen;
+  const V* packs = reinterpret_cast<const V*>(chunk.data);
+  Reduce red;
+  auto add = [&](const V& v) {
+    #pragma unroll
+    for (int j = 0; j < L; ++j) red.add(static_cast<float>(v[j]), j);
+  };
+  chunk.each(
+      [&](uint32_t i) {
+        if (kWide) {
+          V v[4];
+          #pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = packs[i + k * kSpanBlock];
+          #pragma unroll
+          for (int k = 0; k < 4; ++k) add(v[k]);
+        } else {
+          #pragma unroll 1
+          for (int k = 0; k < 4; ++k) add(packs[i + k * kSpanBlock]);
+        }
+      },
+      [&](uint32_t i) { add(packs[i]); },
+      [&](uint32_t i) { red.add(static_cast<float>(chunk.data[i]), 0); });
+  return red.template join<kSpanBlock>(scratch);
+}
 
 // Leaves what it reads in the caches, though streaming past them is faster by
 // itself (148 MB: 26 us for 29): the step that follows reads the gradients
@@ -206,37 +247,41 @@ __global__ __launch_bounds__(kSpanBlock) void grad_norm_partial_kernel(
     const SpanTable table, double* __restrict__ partial, int at,
     const NormEnd end) {
   __shared__ double scratch[kSpanBlock / WAVE_SIZE];
-  using V = typename Pack<T>::type;
-  constexpr int L = Pack<T>::kLen;
-  const Chunk<const T> chunk(table, blockIdx.x);
-  const V* packs = reinterpret_cast<const V*>(chunk.data);
-  Reduce red;
-  auto add = [&](const V& v) {
-    #pragma unroll
-    for (int j = 0; j < L; ++j) red.add(static_cast<float>(v[j]), j);
-  };
-  chunk.each(
-      [&](uint32_t i) {
-        V v[4];
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = packs[i + k * kSpanBlock];
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) add(v[k]);
-      },
-      [&](uint32_t i) { add(packs[i]); },
-      [&](uint32_t i) { red.add(static_cast<float>(chunk.data[i]), 0); });
-  const double sum = red.template join<kSpanBlock>(scratch);
+  const double sum = chunk_sum<T, Reduce, true>(
+      Chunk<const T>(table, blockIdx.x), scratch);
   const int own = at + blockIdx.x;
   if (end.sums == nullptr) {
     if (threadIdx.x == 0) partial[own] = sum;
     return;
   }
-  if (threadIdx.x == 0) store_sum(end.sums + own, sum);
+  if (threadIdx.x == 0) {
+    store_sum(end.sums + own, sum);
+    for (int i = own; i < end.cleared; i += end.all)
+      store_no_sum(end.clear + i);
+  }
   if (own != end.all - 1) return;
-  const double all = join_partials<Reduce, kSpanBlock>(
-      end.all, scratch,
-      TakePartials<kSpanBlock>{end.sums, wall_clock64() + kJoinTicks});
-  if (threadIdx.x == 0) end.out.write(Reduce::norm(all));
+  const uint64_t until = wall_clock64() + end.wait_ticks;
+  for (;;) {
+    int missing = end.all;
+    const double all = join_partials<Reduce, kSpanBlock>(
+        end.all, scratch,
+        AwaitPartials<kSpanBlock>{end.sums, until, &missing});
+    if (!__syncthreads_or(missing < end.all)) {
+      if (threadIdx.x == 0) end.out.write(Reduce::norm(all));
+      return;
+    }
+    // launches before this one have ended, so what is missing is this one's
+    int* least = reinterpret_cast<int*>(scratch);
+    if (threadIdx.x == 0) *least = end.all;
+    __syncthreads();
+    atomicMin(least, missing);
+    __syncthreads();
+    const int place = *least;
+    __syncthreads();
+    const double late = chunk_sum<T, Reduce, false>(
+        Chunk<const T>(table, place - at), scratch);
+    if (threadIdx.x == 0) store_sum(end.sums + place, late);
+  }
 }
 
 // The same from partial results of launches that have ended, in one block.
@@ -365,12 +410,19 @@ void make_tables(SpanGroup& group) {
   }
 }
 
-// Leaves one partial result for each chunk, from partial[at] on or in `sums`.
+// Leaves one partial result for each chunk, from partial[at] on or in
+// `places`.
 void launch_grad_norm_partial(const SpanGroup& group, bool inf,
                               double* partial, int64_t at, int64_t all,
-                              uint64_t* sums, double* full, float* rounded,
+                              const NormPlaces& places, int64_t wait_ticks,
+                              double* full, float* rounded,
                               hipStream_t stream) {
-  const NormEnd end = {sums, static_cast<int>(all), {full, rounded}};
+  const NormEnd end = {places.sums,
+                       places.clear,
+                       static_cast<int>(places.cleared),
+                       static_cast<int>(all),
+                       static_cast<uint64_t>(wait_ticks),
+                       {full, rounded}};
   if (inf)
     launch_partials<LargestMagnitude>(group, partial, at, end, stream);
   else

@@ -132,6 +132,10 @@ __device__ __forceinline__ void store_sum(uint64_t* at, double v) {
                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+__device__ __forceinline__ void store_no_sum(uint64_t* at) {
+  __hip_atomic_store(at, kNoSum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 __device__ __forceinline__ double sum_value(uint64_t bits) {
   return __longlong_as_double(static_cast<long long>(bits));
 }

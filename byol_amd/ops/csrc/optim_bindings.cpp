@@ -21,7 +21,8 @@
 void make_tables(SpanGroup& group);
 void launch_grad_norm_partial(const SpanGroup& group, bool inf,
                               double* partial, int64_t at, int64_t all,
-                              uint64_t* sums, double* full, float* rounded,
+                              const NormPlaces& places, int64_t wait_ticks,
+                              double* full, float* rounded,
                               hipStream_t stream);
 void launch_grad_norm_finish(const double* partial, int64_t n, bool inf,
                              double* full, float* rounded, hipStream_t stream);
@@ -228,21 +229,30 @@ class Gradients {
   std::vector<std::pair<const torch::Tensor*, torch::Tensor>> copies_;
 };
 
-// Places for the sums that a norm's blocks tell each other, "none" in all of
-// them between calls, for the current stream of the current device.  Calls on
-// one stream follow each other, so they share it; calls on other streams have
-// their own, and graphs, which may be replayed on any stream, have none.
+// Places for the sums that a norm's blocks tell each other, for the current
+// stream of the current device: two sets that calls take in turn, "none" in all
+// of a set when a call takes it, as the call between has cleared it.  Calls on
+// one stream follow each other, so they share the sets; calls on other streams
+// have their own, and graphs, which may be replayed on any stream, have none.
 class StreamSums {
  public:
-  static uint64_t* get(hipStream_t stream, int64_t n) {
+  static NormPlaces get(hipStream_t stream, int64_t n) {
     const std::lock_guard<std::mutex> lock(mutex());
     const int device = c10::hip::current_device();
-    auto& sums = all()[{device, stream}];
-    if (!sums.defined() || sums.numel() < n)
-      sums = torch::full(
-          {std::max<int64_t>(2 * n, 4096)}, -1,
+    Sets& sets = all()[{device, stream}];
+    if (!sets.sums.defined() || sets.size < n) {
+      sets.size = std::max<int64_t>(2 * n, 4096);
+      sets.sums = torch::full(
+          {2 * sets.size}, -1,
           torch::TensorOptions().dtype(at::kLong).device(at::kCUDA, device));
-    return reinterpret_cast<uint64_t*>(sums.data_ptr<int64_t>());
+      sets.used = 0;
+    }
+    auto* base = reinterpret_cast<uint64_t*>(sets.sums.data_ptr<int64_t>());
+    sets.next ^= 1;
+    const NormPlaces places = {base + sets.next * sets.size,
+                               base + (sets.next ^ 1) * sets.size, sets.used};
+    sets.used = n;
+    return places;
   }
 
   // After a launch that failed: some places may be taken.
@@ -252,7 +262,13 @@ class StreamSums {
   }
 
  private:
-  using Map = std::map<std::pair<int, hipStream_t>, torch::Tensor>;
+  struct Sets {
+    torch::Tensor sums;
+    int64_t size = 0;  // of one set
+    int64_t used = 0;  // places that the last call took
+    int next = 0;      // the set that it took them from
+  };
+  using Map = std::map<std::pair<int, hipStream_t>, Sets>;
   static std::mutex& mutex() {
     static std::mutex m;
     return m;
@@ -276,7 +292,11 @@ struct Norm {
   const double* full;
 };
 
-Norm norm_of(const Gradients& grads, bool inf, hipStream_t stream) {
+// How long the block that joins a norm's sums waits for them, in 10 ns units.
+constexpr int64_t kNormWaitTicks = 1000000;
+
+Norm norm_of(const Gradients& grads, bool inf, hipStream_t stream,
+             int64_t wait_ticks = kNormWaitTicks) {
   int64_t n = 0;
   for (const auto& g : grads.groups()) n += g.chunks();
   const auto options = torch::TensorOptions().device(grads.device());
@@ -287,29 +307,34 @@ Norm norm_of(const Gradients& grads, bool inf, hipStream_t stream) {
   double* parts = norm.buffer.data_ptr<double>();
   double* full = parts + n;
   norm.full = full;
-  uint64_t* sums =
-      n == 0 || is_capturing(stream) ? nullptr : StreamSums::get(stream, n);
+  NormPlaces places = {nullptr, nullptr, 0};
+  if (n > 0 && !is_capturing(stream)) places = StreamSums::get(stream, n);
   int64_t at = 0;
   for (const auto& g : grads.groups()) {
-    launch_grad_norm_partial(g, inf, parts, at, n, sums, full, rounded,
-                             stream);
+    launch_grad_norm_partial(g, inf, parts, at, n, places, wait_ticks, full,
+                             rounded, stream);
     at += g.chunks();
   }
-  if (sums == nullptr)
+  if (places.sums == nullptr)
     launch_grad_norm_finish(parts, n, inf, full, rounded, stream);
   const hipError_t launched = hipGetLastError();
-  if (launched != hipSuccess && sums != nullptr) StreamSums::forget(stream);
+  if (launched != hipSuccess && places.sums != nullptr) StreamSums::forget(stream);
   C10_HIP_CHECK(launched);
   return norm;
 }
 
-torch::Tensor grad_norm(const pybind11::list& list, bool inf) {
+torch::Tensor grad_norm(const pybind11::list& list, bool inf,
+                        int64_t wait_ticks) {
   const char* what = "global_grad_norm";
+  TORCH_CHECK_VALUE(wait_ticks >= 0 && wait_ticks <= kNormWaitTicks, what,
+                    ": wait_ticks must be 0 to ", kNormWaitTicks, ", got ",
+                    wait_ticks);
   const TensorList tensors(list, what);
   TORCH_CHECK_VALUE(!tensors.empty(), what, ": no tensors");
   const Gradients grads(tensors, what, false);
   const c10::DeviceGuard guard(grads.device());
-  return norm_of(grads, inf, at::hip::getCurrentHIPStream()).rounded;
+  return norm_of(grads, inf, at::hip::getCurrentHIPStream(), wait_ticks)
+      .rounded;
 }
 
 torch::Tensor grad_clip_norm(const pybind11::list& list, double max_norm,
@@ -478,7 +503,9 @@ void lamb_step(const pybind11::list& param_list,
 }  // namespace
 
 void bind_optim(pybind11::module& mod) {
-  mod.def("grad_norm", &grad_norm, "global gradient norm (gfx950)");
+  mod.def("grad_norm", &grad_norm, "global gradient norm (gfx950)",
+          pybind11::arg("grads"), pybind11::arg("inf"),
+          pybind11::arg("wait_ticks") = kNormWaitTicks);
   mod.def("grad_clip_norm", &grad_clip_norm,
           "clip gradients by their global norm (gfx950)");
   mod.def("grad_clip_value", &grad_clip_value,

@@ -26,6 +26,14 @@ struct LambPlan {
   int64_t chunks;
 };
 
+// Where the blocks of a norm tell each other their sums: a call's own places,
+// or null, and those of the call before it on the stream, to be cleared.
+struct NormPlaces {
+  uint64_t* sums;
+  uint64_t* clear;
+  int64_t cleared;
+};
+
 // Element types of a span, as the bindings name them.
 enum class SpanType { kF32, kBF16, kF16 };
 

@@ -545,3 +545,36 @@ def test_captured_with_the_lars_step():
         torch.cuda.synchronize()
         assert torch.equal(norm, expect)
         assert torch.equal(got.flat_params, want.flat_params)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("norm_type", [2.0, math.inf])
+@pytest.mark.parametrize("sizes", [[1], [300_001, 5, 64], [7] * 500,
+                                   [3_000_001, 1, 70_000]])
+def test_norm_of_a_join_that_does_not_wait(norm_type, sizes):
+    """The joining block computes what it would have to wait for: the same
+    bits, and no sum of a late block is left for a later call, whose list is
+    shorter or longer and has other values."""
+    ext, inf = ops.extension(), norm_type == math.inf
+    _, grads = make(sizes, torch.float32, "cuda", gap=1)
+    _, other = make([n // 2 + 1 for n in sizes] + [9], torch.bfloat16, "cuda",
+                    seed=4, gap=1)
+    lists = [grads, other, [2 * g for g in grads], grads + other]
+    want = [ops.global_grad_norm(gs, norm_type) for gs in lists]
+    for gs, norm in zip(lists, want):
+        check_norm(norm, exact_norm(gs, norm_type))
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+        for turn in range(6):
+            for i in (0, 1, 2, 1, 3, 0):
+                ticks = (0, 1, 1000000)[(turn + i) % 3]
+                assert torch.equal(ext.grad_norm(lists[i], inf, ticks),
+                                   want[i]), (turn, i, ticks)
+
+
+@pytest.mark.skipif(not ops.has_extension(), reason="extension not built")
+def test_binding_refuses_waits_out_of_range():
+    g = torch.ones(64)
+    for ticks in (-1, 10 ** 9):
+        with pytest.raises(ValueError, match="wait_ticks"):
+            ops.extension().grad_norm([g], False, ticks)
