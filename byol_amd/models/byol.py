@@ -64,6 +64,10 @@ class FlatParamSpace:
         self.module = module
         self.flat_params: Optional[torch.Tensor] = None
         self.flat_grads: Optional[torch.Tensor] = None
+        # whether FlatDDP reduces flat_grads (it then holds all gradients)
+        self.reduced = False
+        self._grad_views: List[torch.Tensor] = []
+        self._homing = False
         # name -> (offset, numel, shape), in module.named_parameters() order
         self.layout: List[Tuple[str, int, int, torch.Size]] = []
         self.numel = 0
@@ -77,6 +81,7 @@ class FlatParamSpace:
             self.numel, dtype=p0.dtype, device=p0.device)
         self.flat_grads = torch.zeros_like(self.flat_params)
         self.layout = []
+        self._grad_views = []
         offset = 0
         for name, p in params:
             n = p.numel()
@@ -85,6 +90,7 @@ class FlatParamSpace:
             view.copy_(p.detach())
             p.data = view
             p.grad = self.flat_grads[offset:offset + n].view(p.shape)
+            self._grad_views.append(p.grad)
             offset += n
         return self.flat_params
 
@@ -126,6 +132,34 @@ class FlatParamSpace:
 
     def zero_grads(self) -> None:
         self.flat_grads.zero_()
+
+    def attach_grads(self) -> None:
+        """Every parameter that has no gradient gets its view again."""
+        for p, view in zip(self.module.parameters(), self._grad_views):
+            if p.grad is None:
+                p.grad = view
+
+    def drop_grads(self) -> None:
+        """Zero the buffer and leave every ``p.grad`` at ``None``, until a
+        backward pass reaches the parameter: its gradient is the view of the
+        buffer then, as before.  So a parameter that no backward pass reaches
+        is seen to have no gradient, rather than one of zeros."""
+        self.flat_grads.zero_()
+        params = list(self.module.parameters())
+        if not self._homing:
+            for p, view in zip(params, self._grad_views):
+                if p.requires_grad:
+                    p.register_hook(self._make_homing_hook(p, view))
+            self._homing = True
+        for p in params:
+            p.grad = None
+
+    @staticmethod
+    def _make_homing_hook(p, view):
+        def hook(_grad):  # runs before the gradient is accumulated
+            if p.grad is None:
+                p.grad = view
+        return hook
 
     def grad_segments(self) -> List[Tuple[str, int, int]]:
         return [(name, off, n) for name, off, n, _ in self.layout]

@@ -41,18 +41,27 @@ class LAMB(Optimizer):
         return self.defaults.get("max_grad_norm", 0.0)
 
     def attach_flat_space(self, flat_space):
-        """Keep gradients as views of the model's flat buffer, which
-        :class:`~byol_amd.parallel.FlatDDP` reduces: ``zero_grad`` then
-        clears them in place instead of dropping them."""
+        """Keep gradients as views of the model's flat buffer: the kernels
+        pass over it as one tensor, and
+        :class:`~byol_amd.parallel.FlatDDP` reduces it.
+
+        ``zero_grad`` still leaves no gradient behind, and ``step`` skips the
+        parameters that no backward pass reaches.  Where FlatDDP reduces the
+        buffer a parameter may have its gradient from another rank, so there
+        the gradients are cleared in place, and one that no rank reaches
+        counts as zeros: its update is the weight decay alone, which the trust
+        ratio scales to ``lr * |p|`` whatever the decay is."""
         flat_space.verify()
         self._flat_space = flat_space
 
     def zero_grad(self, set_to_none: bool = True):
         space = getattr(self, "_flat_space", None)
-        if space is not None:
-            space.zero_grads()
-        else:
+        if space is None:
             super().zero_grad(set_to_none=set_to_none)
+        elif set_to_none and not space.reduced:
+            space.drop_grads()
+        else:
+            space.zero_grads()
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -61,6 +61,9 @@ class FlatDDP(nn.Module):
         self.module = module
         space = module.flat_space  # requires finalize()d BYOL
         self._space = space
+        # a parameter that has no gradient here may have one on another rank
+        space.reduced = True
+        space.attach_grads()
         self.process_group = process_group
         self.world_size = dist.get_world_size(process_group)
         self.broadcast_buffers = broadcast_buffers

@@ -576,3 +576,93 @@ def test_replicas_stay_alike(lamb, tmp_path):
     for x, y in zip(a["norms"], b["norms"]):
         assert torch.equal(x, y)
     assert all(n <= 0.5 * (1 + 4 * E) for n in a["norms"][1::2])
+
+
+class Branches(torch.nn.Module):
+    """Two layers, of which forward uses the first and, if asked, the other."""
+
+    def __init__(self):
+        super().__init__()
+        self.used = torch.nn.Linear(6, 5)
+        self.unused = torch.nn.Linear(6, 5)
+        self.frozen = torch.nn.Parameter(torch.ones(3), requires_grad=False)
+
+    def forward(self, x, both=False):
+        y = self.used(x)
+        return (y + self.unused(x) if both else y).square().mean()
+
+
+def flat_branches(device, **kw):
+    from byol_amd.models.byol import FlatParamSpace
+    torch.manual_seed(0)
+    net = Branches().to(device)
+    space = FlatParamSpace(net)
+    space.flatten()
+    opt = LAMB(net.parameters(), lr=0.01, weight_decay=1e-4, **kw)
+    opt.attach_flat_space(space)
+    return net, space, opt
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_flat_space_skips_parameters_without_a_gradient(device):
+    net, space, opt = flat_branches(device, max_grad_norm=1.0)
+    x = torch.randn(8, 6, device=device)
+    idle = (net.unused.weight, net.unused.bias, net.frozen)
+    before = [p.detach().clone() for p in idle]
+    moved = net.used.weight.detach().clone()
+    for _ in range(5):
+        opt.zero_grad()
+        assert all(p.grad is None for p in net.parameters())
+        net(x).backward()
+        opt.step()
+    for p, b in zip(idle, before):
+        assert torch.equal(p, b) and p.grad is None and p not in opt.state
+    assert not torch.equal(net.used.weight, moved)
+    # then it is used, and its gradient is where the others are
+    opt.zero_grad()
+    net(x, both=True).backward()
+    net(x, both=True).backward()  # and accumulates there
+    want = torch.autograd.grad(net(x, both=True), list(net.used.parameters())
+                               + list(net.unused.parameters()))
+    for p, g in zip([*net.used.parameters(), *net.unused.parameters()], want):
+        assert torch.allclose(p.grad, 2 * g)
+    space.flat_grads.fill_(2.0)
+    assert all((p.grad == 2).all() for p in net.parameters()
+               if p.requires_grad)
+    opt.step()
+    assert not torch.equal(net.unused.weight, before[0])
+    assert opt.state[net.unused.weight]["step"] == 1
+    assert torch.equal(net.frozen, before[2])
+
+
+def test_flat_space_clears_in_place_if_asked():
+    net, space, opt = flat_branches("cpu")
+    net(torch.randn(8, 6)).backward()
+    opt.zero_grad(set_to_none=False)
+    assert all((p.grad == 0).all() for p in net.parameters())
+    space.flat_grads.fill_(2.0)
+    assert all((p.grad == 2).all() for p in net.parameters())
+
+
+def test_reduced_flat_space_keeps_all_gradients():
+    """FlatDDP fills in gradients from other ranks: none is dropped, also if
+    it wraps the model after an optimizer dropped them."""
+    from byol_amd.parallel.ddp import FlatDDP
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", "29573"
+    dist.init_process_group("gloo", rank=0, world_size=1)
+    try:
+        net, space, opt = flat_branches("cpu")
+        net.frozen.requires_grad_(True)
+        net.flat_space, net.target_network = space, None
+        opt.zero_grad()
+        ddp = FlatDDP(net)
+        for _ in range(2):
+            ddp(torch.randn(8, 6)).backward()
+            ddp.finish_grad_sync()
+            assert all(p.grad is not None for p in net.parameters())
+            opt.step()
+            opt.zero_grad()
+        space.flat_grads.fill_(2.0)
+        assert all((p.grad == 2).all() for p in net.parameters())
+    finally:
+        dist.destroy_process_group()
