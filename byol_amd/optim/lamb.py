@@ -141,8 +141,12 @@ class LAMB(Optimizer):
         beta1, beta2 = group["betas"]
         grad = p.grad
         if norm is not None:
-            grad = grad * (self.max_grad_norm / (norm.double() + 1e-6)) \
-                .clamp(max=1.0).to(grad.dtype)
+            # not in a half-precision gradient's own type: fp16 has no factor
+            # below 3e-8, and bf16 would round twice
+            kind = torch.promote_types(grad.dtype, torch.float32)
+            grad = grad.to(kind) * (
+                self.max_grad_norm / (norm.double() + 1e-6)) \
+                .clamp(max=1.0).to(kind)
         exp_avg, exp_avg_sq = state["exp_avg"], state["exp_avg_sq"]
         exp_avg.mul_(beta1).add_(grad, alpha=1 - beta1)
         exp_avg_sq.mul_(beta2).addcmul_(grad, grad, value=1 - beta2)

@@ -666,3 +666,32 @@ def test_reduced_flat_space_keeps_all_gradients():
         assert all((p.grad == 2).all() for p in net.parameters())
     finally:
         dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,value,bound", [
+    # factors 2.64e-10 and 0.0317
+    (torch.float16, 6e4, 1e-2), (torch.float16, 0.5, 10.0),
+    (torch.bfloat16, 6e4, 1e-2), (torch.bfloat16, 0.5, 10.0)])
+def test_half_precision_parameters_clip_in_fp32(device, dtype, value, bound):
+    """b1 = b2 = 0 puts the clipped gradient and its square in the moments, as
+    they are but for roundings: 3e on g' in fp32 (see above), one to the
+    moment's type and, on the way, one of the product with 1 - b1 = 1; for
+    the square 7e and the same.  Below the type's normal numbers the rounding
+    to it is half of its smallest subnormal instead."""
+    p = torch.nn.Parameter(torch.full((400, 1000), 0.01, dtype=dtype,
+                                      device=device))
+    opt = LAMB([p], lr=0.1, betas=(0.0, 0.0), max_grad_norm=bound)
+    p.grad = torch.full_like(p, value)
+    g = p.grad[0, 0].double().item()
+    want = g * min(1.0, bound / (g * math.sqrt(p.numel()) + 1e-6))
+    opt.step()
+    half = torch.finfo(dtype).eps / 2
+    least = torch.finfo(dtype).tiny * half
+    state = opt.state[p]
+    for name, value, terms in (("exp_avg", want, 4), ("exp_avg_sq", want ** 2,
+                                                      8)):
+        got = state[name].double()
+        off = 1.01 * value * (terms * E + half) + least
+        assert ((got - value).abs() <= off).all(), (name, got[0, 0], value)
+    assert state["exp_avg"].dtype == dtype and p.isfinite().all()
