@@ -14,17 +14,6 @@ from torch.optim.optimizer import Optimizer
 
 __all__ = ["LAMB"]
 
-_GRAD_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-
-
-def _takes_fused_step(p) -> bool:
-    g = p.grad
-    return (p.is_cuda and p.dtype == torch.float32
-            and g.dtype in _GRAD_DTYPES and g.layout is torch.strided
-            and (p.is_contiguous()
-                 or p.is_contiguous(memory_format=torch.channels_last)))
-
-
 class LAMB(Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-6,
                  weight_decay=0.0, max_grad_norm=0.0):
@@ -85,7 +74,7 @@ class LAMB(Optimizer):
                 state["step"] += 1
             lists = (params, grads, [s["exp_avg"] for s in states],
                      [s["exp_avg_sq"] for s in states])
-            if params[0].is_cuda and self._fit_one_step(lists, states):
+            if self._fit_one_step(lists, states):
                 self._add_to_step(fused, group, lists, states[0]["step"])
             else:
                 self._step_each(fused, group, params, states, norm)
@@ -108,7 +97,10 @@ class LAMB(Optimizer):
 
     @staticmethod
     def _fit_one_step(lists, states) -> bool:
-        """Whether a group's tensors can all go into the same fused step."""
+        """Whether a group's tensors can all go into the same fused step.
+        The one rule for it, for a single tensor too."""
+        if not lists[0][0].is_cuda:
+            return False
         from ..ops import require_extension
         return require_extension("LAMB.step").lamb_fits(*lists) \
             and len({s["step"] for s in states}) == 1
@@ -125,17 +117,19 @@ class LAMB(Optimizer):
 
     def _step_each(self, fused, group, params, states, norm):
         for p, state in zip(params, states):
-            if not _takes_fused_step(p):
+            if p.is_cuda and p.dtype == torch.float32 and (
+                    p.is_contiguous() or p.is_contiguous(
+                        memory_format=torch.channels_last)):
+                for name in ("exp_avg", "exp_avg_sq"):
+                    # a checkpoint of another memory format or type
+                    if state[name].stride() != p.stride() \
+                            or state[name].dtype != p.dtype:
+                        state[name] = torch.empty_like(p).copy_(state[name])
+            lists = ([p], [p.grad], [state["exp_avg"]], [state["exp_avg_sq"]])
+            if self._fit_one_step(lists, [state]):
+                self._add_to_step(fused, group, lists, state["step"])
+            else:
                 self._step_one(p, state, group, norm)
-                continue
-            for name in ("exp_avg", "exp_avg_sq"):
-                # a checkpoint of another memory format or type
-                if state[name].stride() != p.stride() \
-                        or state[name].dtype != p.dtype:
-                    state[name] = torch.empty_like(p).copy_(state[name])
-            self._add_to_step(fused, group,
-                              ([p], [p.grad], [state["exp_avg"]],
-                               [state["exp_avg_sq"]]), state["step"])
 
     def _step_one(self, p, state, group, norm):
         beta1, beta2 = group["betas"]

@@ -695,3 +695,46 @@ def test_half_precision_parameters_clip_in_fp32(device, dtype, value, bound):
         off = 1.01 * value * (terms * E + half) + least
         assert ((got - value).abs() <= off).all(), (name, got[0, 0], value)
     assert state["exp_avg"].dtype == dtype and p.isfinite().all()
+
+
+@pytest.mark.gpu
+def test_optimizer_steps_parameters_past_31_bits():
+    """A parameter of 2^31 elements is too long for the fused step; beside
+    one that is not.  With b1 = b2 = eps = 0 and g = 1, u = 1 without a
+    rounding, and r = |p| / |u| = 0.5: sums of powers of two are exact up to
+    2^24 of them, and joining those takes up to 31 roundings."""
+    n = 2 ** 31
+    params = [torch.nn.Parameter(torch.full((k,), 0.5, device="cuda"))
+              for k in (n, 7)]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    opt = LAMB(params, lr=0.5, betas=(0.0, 0.0), eps=0.0)
+    opt.step()
+    for p in params:
+        assert opt.state[p]["step"] == 1
+        low, high = p.detach().aminmax()
+        for got in (low, high):
+            assert abs(got.item() - 0.25) <= 0.25 * 32 * E
+    del params, p, opt
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_optimizer_lays_moments_out_like_their_parameter():
+    """A checkpoint of another memory format, and moments of another type."""
+    gen = torch.Generator().manual_seed(2)
+    w = torch.randn(8, 6, 3, 3, generator=gen)
+    g = torch.randn(8, 6, 3, 3, generator=gen)
+    results = []
+    for spoil in (False, True):
+        p = torch.nn.Parameter(w.cuda().to(memory_format=torch.channels_last))
+        opt = LAMB([p], lr=0.1)
+        for turn in range(2):
+            p.grad = g.cuda()
+            opt.step()
+            if spoil:
+                state = opt.state[p]
+                state["exp_avg"] = state["exp_avg"].contiguous()
+                state["exp_avg_sq"] = state["exp_avg_sq"].double()
+        results.append(p)
+    assert torch.equal(*results)
