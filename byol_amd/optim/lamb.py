@@ -63,6 +63,11 @@ class LAMB(Optimizer):
             params = [p for p in group["params"] if p.grad is not None]
             if params:
                 groups.append((group, params, [p.grad for p in params]))
+        if any(params[0].is_cuda for _, params, _ in groups) \
+                and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("LAMB.step cannot be captured into a graph: "
+                               "its step count and learning rate are host "
+                               "values")
         norm = None
         if self.max_grad_norm > 0 and groups:
             from ..ops import global_grad_norm
@@ -70,12 +75,10 @@ class LAMB(Optimizer):
         fused = {}
         for group, params, grads in groups:
             states = [self._state_of(p) for p in params]
-            for state in states:
-                state["step"] += 1
             lists = (params, grads, [s["exp_avg"] for s in states],
                      [s["exp_avg_sq"] for s in states])
             if self._fit_one_step(lists, states):
-                self._add_to_step(fused, group, lists, states[0]["step"])
+                self._add_to_step(fused, group, lists, states)
             else:
                 self._step_each(fused, group, params, states, norm)
         if fused:
@@ -85,6 +88,9 @@ class LAMB(Optimizer):
                                 eps=eps, weight_decay=lists[4],
                                 max_grad_norm=self.max_grad_norm,
                                 grad_norm=norm)
+                # counted when taken: a refused step leaves the count
+                for state in lists[5]:
+                    state["step"] = step
         return loss
 
     def _state_of(self, p):
@@ -106,14 +112,15 @@ class LAMB(Optimizer):
             and len({s["step"] for s in states}) == 1
 
     @staticmethod
-    def _add_to_step(fused, group, lists, step):
+    def _add_to_step(fused, group, lists, states):
         params, grads = lists[:2]
-        key = (params[0].device, grads[0].dtype, step, group["lr"],
-               tuple(group["betas"]), group["eps"])
-        all_lists = fused.setdefault(key, ([], [], [], [], []))
+        key = (params[0].device, grads[0].dtype, states[0]["step"] + 1,
+               group["lr"], tuple(group["betas"]), group["eps"])
+        all_lists = fused.setdefault(key, ([], [], [], [], [], []))
         for values, more in zip(all_lists, lists):
             values.extend(more)
         all_lists[4].extend([max(group["weight_decay"], 0.0)] * len(params))
+        all_lists[5].extend(states)
 
     def _step_each(self, fused, group, params, states, norm):
         for p, state in zip(params, states):
@@ -127,7 +134,7 @@ class LAMB(Optimizer):
                         state[name] = torch.empty_like(p).copy_(state[name])
             lists = ([p], [p.grad], [state["exp_avg"]], [state["exp_avg_sq"]])
             if self._fit_one_step(lists, [state]):
-                self._add_to_step(fused, group, lists, state["step"])
+                self._add_to_step(fused, group, lists, [state])
             else:
                 self._step_one(p, state, group, norm)
 
@@ -144,6 +151,7 @@ class LAMB(Optimizer):
         exp_avg, exp_avg_sq = state["exp_avg"], state["exp_avg_sq"]
         exp_avg.mul_(beta1).add_(grad, alpha=1 - beta1)
         exp_avg_sq.mul_(beta2).addcmul_(grad, grad, value=1 - beta2)
+        state["step"] += 1
         bias1 = 1 - beta1 ** state["step"]
         bias2 = 1 - beta2 ** state["step"]
         update = (exp_avg / bias1) / (

@@ -738,3 +738,42 @@ def test_optimizer_lays_moments_out_like_their_parameter():
                 state["exp_avg_sq"] = state["exp_avg_sq"].double()
         results.append(p)
     assert torch.equal(*results)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_optimizer_counts_only_steps_that_it_takes(device, monkeypatch):
+    p = torch.nn.Parameter(torch.ones(6, device=device))
+    opt = LAMB([p], lr=0.1)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    before = p.detach().clone()
+
+    def refuse(*args, **kw):
+        raise ValueError("refused")
+    with monkeypatch.context() as patch:
+        patch.setattr(ops, "fused_lamb_step", refuse)
+        patch.setattr(LAMB, "_fit_one_step", staticmethod(lambda *a: True))
+        with pytest.raises(ValueError, match="refused"):
+            opt.step()
+    assert opt.state[p]["step"] == 1 and torch.equal(p, before)
+    opt.step()
+    assert opt.state[p]["step"] == 2
+
+
+@pytest.mark.gpu
+def test_optimizer_refuses_capture_before_it_does_anything():
+    half = torch.nn.Parameter(torch.ones(6, device="cuda").bfloat16())
+    p = torch.nn.Parameter(torch.ones(6, device="cuda"))
+    opt = LAMB([half, p], lr=0.1, max_grad_norm=1.0)
+    for t in (half, p):
+        t.grad = torch.ones_like(t)
+    opt.step()
+    before = [t.detach().clone() for t in (half, p)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()
+        p.grad.mul_(1.0)
+    torch.cuda.synchronize()
+    for t, b in zip((half, p), before):
+        assert torch.equal(t, b) and opt.state[t]["step"] == 1
