@@ -113,11 +113,13 @@ class Ranges {
     ranges_.push_back(r);
   }
 
-  void check_disjoint(const char* what) {
+  // Sorts the ranges; whether no two of them meet.
+  bool disjoint() {
     if (!ordered_) std::sort(ranges_.begin(), ranges_.end());
+    ordered_ = true;
     for (size_t i = 1; i < ranges_.size(); ++i)
-      TORCH_CHECK_VALUE(ranges_[i - 1].second <= ranges_[i].first, what,
-                        ": a tensor is listed twice, or two share memory");
+      if (ranges_[i - 1].second > ranges_[i].first) return false;
+    return true;
   }
 
   // Whether none of the (disjoint) ranges reaches into `t`'s.
@@ -171,7 +173,8 @@ class Gradients {
           "cannot be written in place");
       ranges.add(list[i]);
     }
-    if (write) ranges.check_disjoint(what);
+    TORCH_CHECK_VALUE(!write || ranges.disjoint(), what,
+                      ": a tensor is listed twice, or two share memory");
     check_device(list, what, device_);
     const c10::DeviceGuard guard(device_);
     for (size_t i = 0; i < n; ++i) {
@@ -407,13 +410,16 @@ bool lamb_fits(const pybind11::list& param_list,
   return true;
 }
 
-void lamb_step(const pybind11::list& param_list,
+// Returns false, and has written nothing, where tensors share memory, if that
+// is not to raise.
+bool lamb_step(const pybind11::list& param_list,
                const pybind11::list& grad_list,
                const pybind11::list& exp_avg_list,
                const pybind11::list& exp_avg_sq_list,
                const std::vector<double>& decay, int64_t step, double lr,
                double beta1, double beta2, double eps, double max_norm,
-               const c10::optional<torch::Tensor>& norm, int64_t wait_ticks) {
+               const c10::optional<torch::Tensor>& norm, int64_t wait_ticks,
+               bool refuse_shared) {
   const char* what = "fused_lamb_step";
   const TensorList params(param_list, what), grads(grad_list, what),
       exp_avgs(exp_avg_list, what), exp_avg_sqs(exp_avg_sq_list, what);
@@ -424,7 +430,7 @@ void lamb_step(const pybind11::list& param_list,
   TORCH_CHECK_VALUE(step >= 1, what, ": step counts from 1, got ", step);
   TORCH_CHECK_VALUE(wait_ticks >= 0 && wait_ticks <= 100000, what,
                     ": wait_ticks must be 0 to 100000, got ", wait_ticks);
-  if (n == 0) return;
+  if (n == 0) return true;
   Ranges written(3 * n);
   for (const auto* list : {&params, &exp_avgs, &exp_avg_sqs}) {
     for (size_t i = 0; i < n; ++i) {
@@ -450,11 +456,18 @@ void lamb_step(const pybind11::list& param_list,
     TORCH_CHECK_VALUE(grads[i].sizes() == params[i].sizes(), what,
                       ": a gradient has another shape than its parameter");
   }
-  written.check_disjoint(what);
-  for (size_t i = 0; i < n; ++i)
-    TORCH_CHECK_VALUE(written.apart_from(grads[i]), what,
+  if (!written.disjoint()) {
+    TORCH_CHECK_VALUE(!refuse_shared, what,
+                      ": a tensor is listed twice, or two share memory");
+    return false;
+  }
+  for (size_t i = 0; i < n; ++i) {
+    if (written.apart_from(grads[i])) continue;
+    TORCH_CHECK_VALUE(!refuse_shared, what,
                       ": a gradient shares memory with a parameter or a "
                       "moment");
+    return false;
+  }
   const auto device = params[0].device();
   for (const auto* list : {&params, &grads, &exp_avgs, &exp_avg_sqs})
     check_device(*list, what, device);
@@ -484,7 +497,7 @@ void lamb_step(const pybind11::list& param_list,
                     exp_avg_sqs[i].data_ptr<float>(), p.numel(),
                     static_cast<float>(decay[i])});
   }
-  if (list.empty()) return;
+  if (list.empty()) return true;
   const LambPlan plan = lamb_plan(list);
   TORCH_CHECK_VALUE(plan.chunks < (int64_t(1) << 30), what, ": too many elements");
   auto workspace = torch::empty(
@@ -498,6 +511,7 @@ void lamb_step(const pybind11::list& param_list,
   mark_written(params);
   mark_written(exp_avgs);
   mark_written(exp_avg_sqs);
+  return true;
 }
 
 }  // namespace
@@ -520,5 +534,6 @@ void bind_optim(pybind11::module& mod) {
           pybind11::arg("norm") = pybind11::none(),
           // how long a block waits for the others of its tensor, in 10 ns
           // units; without a wait all long tensors take the second pass
-          pybind11::arg("wait_ticks") = 20000);
+          pybind11::arg("wait_ticks") = 20000,
+          pybind11::arg("refuse_shared") = true);
 }

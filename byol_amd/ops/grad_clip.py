@@ -58,22 +58,27 @@ def _on_gpu(grads: Sequence[torch.Tensor], what: str) -> bool:
     return False
 
 
+class SharedMemoryError(ValueError):
+    """Tensors that are written share memory."""
+
+
 def check_writable(grads: Sequence[torch.Tensor], what: str) -> None:
     ranges = []
     for t in grads:
         if t.numel() == 0:
             continue
         if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-            raise ValueError(f"{what}: elements of a tensor share memory (an "
-                             "expanded view); it cannot be written in place")
+            raise SharedMemoryError(f"{what}: elements of a tensor share memory "
+                                    "(an expanded view); it cannot be written "
+                                    "in place")
         reach = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
         ranges.append((t.data_ptr(),
                        t.data_ptr() + reach * t.element_size()))
     ranges.sort()
     for a, b in zip(ranges, ranges[1:]):
         if a[1] > b[0]:
-            raise ValueError(f"{what}: a tensor is listed twice, or two "
-                             "share memory")
+            raise SharedMemoryError(f"{what}: a tensor is listed twice, or "
+                                    "two share memory")
 
 
 def _reference_norm(grads, inf: bool) -> torch.Tensor:

@@ -18,7 +18,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import require_extension
-from .grad_clip import check_writable, global_grad_norm
+from .grad_clip import SharedMemoryError, check_writable, global_grad_norm
 
 __all__ = ["fused_lamb_step"]
 
@@ -77,9 +77,12 @@ def fused_lamb_step(params: Sequence[torch.Tensor],
     if max_grad_norm == 0:
         grad_norm = None
     if on_gpu:
-        require_extension("fused_lamb_step").lamb_step(
-            params, grads, exp_avgs, exp_avg_sqs, decay, step, lr, b1, b2,
-            eps, max_grad_norm, grad_norm)
+        if not require_extension("fused_lamb_step").lamb_step(
+                params, grads, exp_avgs, exp_avg_sqs, decay, step, lr, b1, b2,
+                eps, max_grad_norm, grad_norm, refuse_shared=False):
+            raise SharedMemoryError(
+                "fused_lamb_step: a tensor is listed twice, or two share "
+                "memory")
         return
     _reference_step(params, grads, exp_avgs, exp_avg_sqs, decay, step, lr,
                     b1, b2, eps, max_grad_norm, grad_norm)

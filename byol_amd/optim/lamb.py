@@ -83,11 +83,17 @@ class LAMB(Optimizer):
                 self._step_each(fused, group, params, states, norm)
         if fused:
             from ..ops import fused_lamb_step
+            from ..ops.grad_clip import SharedMemoryError
             for (_, _, step, lr, betas, eps), lists in fused.items():
-                fused_lamb_step(*lists[:4], step=step, lr=lr, betas=betas,
-                                eps=eps, weight_decay=lists[4],
-                                max_grad_norm=self.max_grad_norm,
-                                grad_norm=norm)
+                try:
+                    fused_lamb_step(*lists[:4], step=step, lr=lr, betas=betas,
+                                    eps=eps, weight_decay=lists[4],
+                                    max_grad_norm=self.max_grad_norm,
+                                    grad_norm=norm)
+                except SharedMemoryError:  # nothing has been written
+                    for p, state, group in zip(lists[0], *lists[5:]):
+                        self._step_one(p, state, group, norm)
+                    continue
                 # counted when taken: a refused step leaves the count
                 for state in lists[5]:
                     state["step"] = step
@@ -116,11 +122,12 @@ class LAMB(Optimizer):
         params, grads = lists[:2]
         key = (params[0].device, grads[0].dtype, states[0]["step"] + 1,
                group["lr"], tuple(group["betas"]), group["eps"])
-        all_lists = fused.setdefault(key, ([], [], [], [], [], []))
+        all_lists = fused.setdefault(key, tuple([] for _ in range(7)))
         for values, more in zip(all_lists, lists):
             values.extend(more)
         all_lists[4].extend([max(group["weight_decay"], 0.0)] * len(params))
         all_lists[5].extend(states)
+        all_lists[6].extend([group] * len(params))
 
     def _step_each(self, fused, group, params, states, norm):
         for p, state in zip(params, states):

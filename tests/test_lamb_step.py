@@ -777,3 +777,46 @@ def test_optimizer_refuses_capture_before_it_does_anything():
     torch.cuda.synchronize()
     for t, b in zip((half, p), before):
         assert torch.equal(t, b) and opt.state[t]["step"] == 1
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_optimizer_steps_parameters_that_share_memory(device, monkeypatch):
+    """One after the other, in torch operations: the bits of a list that is
+    taken so in any case."""
+    from byol_amd.ops.grad_clip import SharedMemoryError
+
+    def stepped(alone, decay=(0.01, 0.0)):
+        gen = torch.Generator().manual_seed(5)
+        base = torch.randn(50, generator=gen).to(device)
+        params = [torch.nn.Parameter(t) for t in (base[:30], base[20:],
+                                                  base[:7].clone())]
+        opt = LAMB([{"params": params[:2], "weight_decay": decay[0]},
+                    {"params": params[2:], "weight_decay": decay[1]}], lr=0.1,
+                   max_grad_norm=0.5)
+        with monkeypatch.context() as patch:
+            if alone:
+                patch.setattr(LAMB, "_fit_one_step",
+                              staticmethod(lambda *a: False))
+            elif device == "cpu":  # the route that lists on a GPU take
+                def refuse(*args, **kw):
+                    raise SharedMemoryError("two share memory")
+                patch.setattr(ops, "fused_lamb_step", refuse)
+                patch.setattr(LAMB, "_fit_one_step",
+                              staticmethod(lambda *a: True))
+            for _ in range(3):
+                for p in params:
+                    p.grad = torch.randn(p.shape, generator=gen).to(device)
+                opt.step()
+        assert [opt.state[p]["step"] for p in params] == [3, 3, 3]
+        return base, params[2]
+
+    for a, b in zip(stepped(False), stepped(True)):
+        assert torch.equal(a, b) and a.isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sharing_is_refused_as_such(device):
+    from byol_amd.ops.grad_clip import SharedMemoryError
+    _, (p, g, m, v) = make([64, 8], device)
+    with pytest.raises(SharedMemoryError, match="twice"):
+        ops.fused_lamb_step(p, g, m, m, step=1, lr=0.1)
