@@ -14,6 +14,25 @@ from torch.optim.optimizer import Optimizer
 
 __all__ = ["LAMB"]
 
+_GRAD_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+def _norm_of(grads) -> torch.Tensor:
+    """The 2-norm of all gradients; those that the operator does not take in
+    one list (other types, several devices) are joined in fp64."""
+    from ..ops import global_grad_norm
+    device = grads[0].device
+    if len({g.device for g in grads}) == 1 \
+            and {g.dtype for g in grads} <= set(_GRAD_DTYPES):
+        return global_grad_norm(grads)
+    return torch.stack([g.double().square().sum().to(device)
+                        for g in grads]).sum().sqrt()
+
+
+def _on(norm, device):
+    """The norm as the fused step reads it."""
+    return None if norm is None else norm.to(device, torch.float32)
+
+
 class LAMB(Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-6,
                  weight_decay=0.0, max_grad_norm=0.0):
@@ -70,8 +89,7 @@ class LAMB(Optimizer):
                                "values")
         norm = None
         if self.max_grad_norm > 0 and groups:
-            from ..ops import global_grad_norm
-            norm = global_grad_norm([g for _, _, gs in groups for g in gs])
+            norm = _norm_of([g for _, _, gs in groups for g in gs])
         fused = {}
         for group, params, grads in groups:
             states = [self._state_of(p) for p in params]
@@ -89,7 +107,7 @@ class LAMB(Optimizer):
                     fused_lamb_step(*lists[:4], step=step, lr=lr, betas=betas,
                                     eps=eps, weight_decay=lists[4],
                                     max_grad_norm=self.max_grad_norm,
-                                    grad_norm=norm)
+                                    grad_norm=_on(norm, lists[0][0].device))
                 except SharedMemoryError:  # nothing has been written
                     for p, state, group in zip(lists[0], *lists[5:]):
                         self._step_one(p, state, group, norm)
@@ -154,7 +172,7 @@ class LAMB(Optimizer):
             kind = torch.promote_types(grad.dtype, torch.float32)
             grad = grad.to(kind) * (
                 self.max_grad_norm / (norm.double() + 1e-6)) \
-                .clamp(max=1.0).to(kind)
+                .clamp(max=1.0).to(grad.device, kind)
         exp_avg, exp_avg_sq = state["exp_avg"], state["exp_avg_sq"]
         exp_avg.mul_(beta1).add_(grad, alpha=1 - beta1)
         exp_avg_sq.mul_(beta2).addcmul_(grad, grad, value=1 - beta2)

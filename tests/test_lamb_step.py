@@ -820,3 +820,45 @@ def test_sharing_is_refused_as_such(device):
     _, (p, g, m, v) = make([64, 8], device)
     with pytest.raises(SharedMemoryError, match="twice"):
         ops.fused_lamb_step(p, g, m, m, step=1, lr=0.1)
+
+
+def clipped_alike(devices, dtypes):
+    """Gradients of several types or devices are clipped by their common norm:
+    as much as after clipping them by hand."""
+    gen = torch.Generator().manual_seed(6)
+    values = [torch.randn(40, 9, generator=gen) for _ in dtypes]
+    want = math.sqrt(sum(v.to(t).double().square().sum().item()
+                         for v, t in zip(values, dtypes)))
+    results = []
+    for inside in (True, False):
+        params = [torch.nn.Parameter(torch.full((40, 9), 0.1, dtype=t,
+                                                device=d))
+                  for t, d in zip(dtypes, devices)]
+        opt = LAMB(params, lr=0.1, betas=(0.5, 0.5),
+                   max_grad_norm=0.25 if inside else 0.0)
+        for p, v in zip(params, values):
+            p.grad = v.to(p.device, p.dtype)
+            if not inside:
+                p.grad.mul_(0.25 / (want + 1e-6))
+        opt.step()
+        results.append([opt.state[p]["exp_avg"].double().cpu()
+                        for p in params])
+    for a, b, t in zip(*results, dtypes):
+        # both: factor, product and moment; fp64's norm is summed in fp64
+        e = 2.0 ** -52 if t is torch.float64 else max(
+            E, torch.finfo(t).eps / 2)
+        assert ((a - b).abs() <= 8 * e * b.abs()).all()
+
+
+def test_optimizer_clips_fp64():
+    clipped_alike(["cpu"] * 2, [torch.float64] * 2)
+
+
+def test_optimizer_clips_fp64_beside_fp32():
+    clipped_alike(["cpu"] * 2, [torch.float64, torch.float32])
+
+
+@pytest.mark.gpu
+def test_optimizer_clips_on_several_devices():
+    clipped_alike(["cuda", "cpu", "cuda"],
+                  [torch.float32, torch.float32, torch.float64])
