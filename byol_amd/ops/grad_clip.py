@@ -129,13 +129,18 @@ def clip_grads_by_norm_(grads: Sequence[torch.Tensor], max_norm: float,
         return norm.float()
 
 
+def check_clip_value(clip_value: float) -> float:
+    clip_value = float(clip_value)
+    if not clip_value >= 0:
+        raise ValueError(f"clip_value must be >= 0, got {clip_value}")
+    return clip_value
+
+
 def clip_grads_by_value_(grads: Sequence[torch.Tensor],
                          clip_value: float) -> None:
     """Bound every element to ``[-clip_value, clip_value]`` in place; NaN
     stays."""
-    clip_value = float(clip_value)
-    if not clip_value >= 0:
-        raise ValueError(f"clip_value must be >= 0, got {clip_value}")
+    clip_value = check_clip_value(clip_value)
     grads = _as_list(grads)
     if not grads:
         return

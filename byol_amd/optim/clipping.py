@@ -1,8 +1,11 @@
 """Gradient clipping over a model's parameters, by global norm or by value.
 
-Drop-in for the two functions of ``torch.nn.utils``: the gradients of all
+The calls of ``torch.nn.utils``, without its ``foreach``: the gradients of all
 parameters that have one are handed to the fused operators of
-:mod:`byol_amd.ops.grad_clip`.  Under data parallelism call them after the
+:mod:`byol_amd.ops.grad_clip`.  Those take fp32, bf16 and fp16 gradients on one
+device, no two of which reach into each other's memory.  By value, other
+gradients are bounded one by one in torch operations; by norm they are refused,
+and so are norms other than 2 and inf.  Under data parallelism call them after the
 gradients are synchronised (``FlatDDP.finish_grad_sync``): every replica then
 computes the same norm from the same values, without another collective.
 """
@@ -10,6 +13,7 @@ computes the same norm from the same values, without another collective.
 import torch
 
 from ..ops import clip_grads_by_norm_, clip_grads_by_value_
+from ..ops.grad_clip import check_clip_value
 
 __all__ = ["clip_grad_norm_", "clip_grad_value_"]
 
@@ -45,4 +49,12 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
 @torch.no_grad()
 def clip_grad_value_(parameters, clip_value: float) -> None:
     """Bound every gradient value to ``[-clip_value, clip_value]``."""
-    clip_grads_by_value_(_grads(parameters), clip_value)
+    clip_value = check_clip_value(clip_value)
+    grads = _grads(parameters)
+    try:
+        clip_grads_by_value_(grads, clip_value)
+    except (TypeError, ValueError):
+        # a list that the operator does not take; it has written nothing, and
+        # to bound a value twice is to bound it
+        for g in grads:
+            g.clamp_(-clip_value, clip_value)

@@ -578,3 +578,55 @@ def test_binding_refuses_waits_out_of_range():
     for ticks in (-1, 10 ** 9):
         with pytest.raises(ValueError, match="wait_ticks"):
             ops.extension().grad_norm([g], False, ticks)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_parameters_with_gradients_of_any_kind_by_value(device):
+    """What the operator refuses is bounded one by one: fp64, views that
+    interleave or are the same memory, and fp32 beside them."""
+    gen = torch.Generator().manual_seed(8)
+    base = torch.randn(40, generator=gen)
+    plain, double = torch.randn(9, generator=gen), torch.randn(
+        7, generator=gen).double()
+
+    def grads():
+        b = base.to(device)
+        return [b[::2], b[1::2], b[4:9]], [plain.to(device),
+                                           double.to(device)]
+
+    for part in range(2):
+        values = grads()[part]
+        want = [g.clamp(-0.25, 0.25) for g in grads()[part]]
+        params = [torch.nn.Parameter(torch.zeros_like(g)) for g in values]
+        for p, g in zip(params, values):
+            p.grad = g
+        clip_grad_value_(params, 0.25)
+        for p, w in zip(params, want):
+            assert torch.equal(p.grad, w) and p.grad.dtype == w.dtype
+        for bad in (-1.0, math.nan):
+            with pytest.raises(ValueError, match="must be >= 0"):
+                clip_grad_value_(params, bad)
+        for p, w in zip(params, want):
+            assert torch.equal(p.grad, w)
+
+
+@pytest.mark.gpu
+def test_parameters_on_several_devices_by_value():
+    params = [torch.nn.Parameter(torch.zeros(5, device=d))
+              for d in ("cpu", "cuda")]
+    for p in params:
+        p.grad = torch.full_like(p, 3.0)
+    clip_grad_value_(params, 0.5)
+    assert all((p.grad == 0.5).all() for p in params)
+
+
+@pytest.mark.gpu
+def test_missing_extension_is_an_error(monkeypatch):
+    """No fallback hides that the kernels are not built."""
+    def missing(what):
+        raise RuntimeError("not built")
+    monkeypatch.setattr("byol_amd.ops.grad_clip.require_extension", missing)
+    p = torch.nn.Parameter(torch.zeros(5, device="cuda"))
+    p.grad = torch.ones_like(p)
+    with pytest.raises(RuntimeError, match="not built"):
+        clip_grad_value_([p], 0.5)
