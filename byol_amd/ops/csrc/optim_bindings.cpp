@@ -237,12 +237,22 @@ class Gradients {
 // of a set when a call takes it, as the call between has cleared it.  Calls on
 // one stream follow each other, so they share the sets; calls on other streams
 // have their own, and graphs, which may be replayed on any stream, have none.
+// The sets of so many streams are kept, those of the least recent call go: a
+// program may make and drop streams without end.  The memory returns to its
+// stream's pool, behind the calls that use it.
 class StreamSums {
  public:
   static NormPlaces get(hipStream_t stream, int64_t n) {
     const std::lock_guard<std::mutex> lock(mutex());
     const int device = c10::hip::current_device();
+    if (all().size() == kStreams && all().count({device, stream}) == 0)
+      all().erase(std::min_element(
+          all().begin(), all().end(), [](const auto& a, const auto& b) {
+            return a.second.turn < b.second.turn;
+          }));
     Sets& sets = all()[{device, stream}];
+    static uint64_t turns = 0;
+    sets.turn = ++turns;
     if (!sets.sums.defined() || sets.size < n) {
       sets.size = std::max<int64_t>(2 * n, 4096);
       sets.sums = torch::full(
@@ -258,6 +268,11 @@ class StreamSums {
     return places;
   }
 
+  static size_t count() {
+    const std::lock_guard<std::mutex> lock(mutex());
+    return all().size();
+  }
+
   // After a launch that failed: some places may be taken.
   static void forget(hipStream_t stream) {
     const std::lock_guard<std::mutex> lock(mutex());
@@ -265,11 +280,13 @@ class StreamSums {
   }
 
  private:
+  static constexpr size_t kStreams = 16;
   struct Sets {
     torch::Tensor sums;
     int64_t size = 0;  // of one set
     int64_t used = 0;  // places that the last call took
     int next = 0;      // the set that it took them from
+    uint64_t turn = 0;
   };
   using Map = std::map<std::pair<int, hipStream_t>, Sets>;
   static std::mutex& mutex() {
@@ -520,6 +537,8 @@ void bind_optim(pybind11::module& mod) {
   mod.def("grad_norm", &grad_norm, "global gradient norm (gfx950)",
           pybind11::arg("grads"), pybind11::arg("inf"),
           pybind11::arg("wait_ticks") = kNormWaitTicks);
+  mod.def("grad_norm_streams", &StreamSums::count,
+          "streams that places for a norm's sums are kept for");
   mod.def("grad_clip_norm", &grad_clip_norm,
           "clip gradients by their global norm (gfx950)");
   mod.def("grad_clip_value", &grad_clip_value,

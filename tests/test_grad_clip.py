@@ -630,3 +630,24 @@ def test_missing_extension_is_an_error(monkeypatch):
     p.grad = torch.ones_like(p)
     with pytest.raises(RuntimeError, match="not built"):
         clip_grad_value_([p], 0.5)
+
+
+@pytest.mark.gpu
+def test_places_are_kept_for_some_streams_only():
+    """Over more streams than places are kept for, twice over: every norm is
+    right, whether its stream's places are there, gone or in the way."""
+    lists = [make([n, 30_000], torch.float32, "cuda", seed=n)[1]
+             for n in (5, 200_000)]
+    want = [exact_norm(gs, 2.0) for gs in lists]
+    streams = [torch.cuda.Stream() for _ in range(30)]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i + turn, ops.global_grad_norm(
+                    lists[(i + turn) % 2])))
+    torch.cuda.synchronize()
+    for i, norm in got:
+        check_norm(norm, want[i % 2])
+    assert ops.extension().grad_norm_streams() <= 16
