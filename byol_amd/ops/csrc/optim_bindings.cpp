@@ -254,10 +254,11 @@ class StreamSums {
     static uint64_t turns = 0;
     sets.turn = ++turns;
     if (!sets.sums.defined() || sets.size < n) {
-      sets.size = std::max<int64_t>(2 * n, 4096);
+      const int64_t size = std::max<int64_t>(2 * n, 4096);
       sets.sums = torch::full(
-          {2 * sets.size}, -1,
+          {2 * size}, -1,
           torch::TensorOptions().dtype(at::kLong).device(at::kCUDA, device));
+      sets.size = size;  // not if there was no memory for them
       sets.used = 0;
     }
     auto* base = reinterpret_cast<uint64_t*>(sets.sums.data_ptr<int64_t>());
