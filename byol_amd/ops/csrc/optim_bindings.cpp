@@ -145,6 +145,9 @@ bool same_layout(const torch::Tensor& a, const torch::Tensor& b) {
   return true;
 }
 
+// A view may stand for its memory's values negated (is_neg).  The norm and both
+// clippings are the same for the two signs; the LAMB step is not.
+
 // The kernels write through raw pointers: tell autograd, as an in-place
 // operation does.
 void mark_written(const TensorList& list) {
@@ -422,6 +425,7 @@ bool lamb_fits(const pybind11::list& param_list,
     for (const auto* t : {&p, &exp_avgs[i], &exp_avg_sqs[i]})
       if (t->layout() != at::kStrided || t->scalar_type() != at::kFloat ||
           t->device() != device || !t->is_non_overlapping_and_dense() ||
+          t->is_neg() ||
           t->sizes() != p.sizes() || !same_layout(*t, p))
         return false;
   }
@@ -457,7 +461,7 @@ bool lamb_step(const pybind11::list& param_list,
       TORCH_CHECK_TYPE(span_type(t, what) == SpanType::kF32, what,
                        ": parameters and moments must be fp32, got ",
                        t.scalar_type());
-      TORCH_CHECK_VALUE(t.is_non_overlapping_and_dense(), what,
+      TORCH_CHECK_VALUE(t.is_non_overlapping_and_dense() && !t.is_neg(), what,
                         ": parameters and moments must be dense");
       TORCH_CHECK_VALUE(t.numel() < (int64_t(1) << 31), what,
                         ": a parameter has 2^31 elements or more");
@@ -498,14 +502,15 @@ bool lamb_step(const pybind11::list& param_list,
     norm_ptr = norm->data_ptr<float>();
   }
   const c10::DeviceGuard guard(device);
-  std::vector<torch::Tensor> held;  // gradients in their parameters' layout
+  // gradients in their parameters' layout, with the signs that they stand for
+  std::vector<torch::Tensor> held;
   std::vector<LambTensor> list;
   list.reserve(n);
   for (size_t i = 0; i < n; ++i) {
     const auto& p = params[i];
     if (p.numel() == 0) continue;
     const void* g = grads[i].const_data_ptr();
-    if (!same_layout(grads[i], p)) {
+    if (!same_layout(grads[i], p) || grads[i].is_neg()) {
       held.push_back(torch::empty_strided(
           p.sizes(), p.strides(), grads[i].options().requires_grad(false)));
       held.back().copy_(grads[i].detach());

@@ -862,3 +862,41 @@ def test_optimizer_clips_fp64_beside_fp32():
 def test_optimizer_clips_on_several_devices():
     clipped_alike(["cuda", "cpu", "cuda"],
                   [torch.float32, torch.float32, torch.float64])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_views_of_negated_memory(device):
+    """Gradients that are lazily negated views count with their sign; such
+    parameters are refused by the operator on a GPU and stepped by LAMB."""
+    _, lists = make([300, 41], device)
+    before = [[t.clone() for t in ts] for ts in lists]
+    lists[1] = [torch._neg_view(-g) for g in lists[1]]
+    ops.fused_lamb_step(*lists, step=3, lr=0.1, max_grad_norm=0.5)
+    norm = torch.cat([g.cpu().double() for g in before[1]]).norm().item()
+    check(lists, before, 3, 0.1, 1e-6, [0.0, 0.0], 0.5 / (norm + 1e-6),
+          slack=device == "cpu")
+    results = []
+    for negated in (False, True):
+        value = torch.arange(1.0, 9.0, device=device)
+        p = torch.nn.Parameter(torch._neg_view(-value) if negated else value)
+        opt = LAMB([p], lr=0.1)
+        p.grad = torch.ones(8, device=device)
+        opt.step()
+        results.append(p.detach().clone())
+    # the fused form and the one in torch operations: see the bounds above
+    assert torch.allclose(*results, rtol=64 * E, atol=0)
+
+
+@pytest.mark.gpu
+def test_clipping_views_of_negated_memory():
+    g = torch.randn(500, device="cuda")
+    view, before = torch._neg_view(-g), g.clone()
+    norm = before.cpu().double().norm().item()
+    ops.clip_grads_by_norm_([view], norm / 2)
+    want = before.cpu().double() * (norm / 2 / (norm + 1e-6))
+    # the factor and the product are rounded
+    assert ((view.cpu().double() - want).abs()
+            <= 1.01 * 2 * E * want.abs()).all()
+    ops.clip_grads_by_value_([view], 0.25)
+    assert torch.equal(view.sign(), before.sign())
+    assert view.abs().max() == 0.25
