@@ -19,6 +19,7 @@ infinities propagate: an infinite norm scales finite gradients to zero, a NaN
 norm makes all of them NaN.  Nothing here is differentiated through.
 """
 
+import bisect
 import math
 from typing import Sequence
 
@@ -62,7 +63,16 @@ class SharedMemoryError(ValueError):
     """Tensors that are written share memory."""
 
 
-def check_writable(grads: Sequence[torch.Tensor], what: str) -> None:
+def _reach(t: torch.Tensor):
+    """The memory from a tensor's first element to its last."""
+    n = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def check_writable(grads: Sequence[torch.Tensor], what: str,
+                   read: Sequence[torch.Tensor] = ()) -> None:
+    """Refuse tensors that are written and share memory, among each other or
+    with those that are `read`."""
     ranges = []
     for t in grads:
         if t.numel() == 0:
@@ -71,14 +81,20 @@ def check_writable(grads: Sequence[torch.Tensor], what: str) -> None:
             raise SharedMemoryError(f"{what}: elements of a tensor share memory "
                                     "(an expanded view); it cannot be written "
                                     "in place")
-        reach = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        ranges.append((t.data_ptr(),
-                       t.data_ptr() + reach * t.element_size()))
+        ranges.append(_reach(t))
     ranges.sort()
     for a, b in zip(ranges, ranges[1:]):
         if a[1] > b[0]:
             raise SharedMemoryError(f"{what}: a tensor is listed twice, or "
                                     "two share memory")
+    for t in read:
+        if t.numel() == 0:
+            continue
+        begin, end = _reach(t)
+        at = bisect.bisect_left(ranges, (end, 0))
+        if at > 0 and ranges[at - 1][1] > begin:
+            raise SharedMemoryError(f"{what}: a tensor that is read shares "
+                                    "memory with one that is written")
 
 
 def _reference_norm(grads, inf: bool) -> torch.Tensor:

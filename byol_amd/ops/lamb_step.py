@@ -47,7 +47,7 @@ def fused_lamb_step(params: Sequence[torch.Tensor],
     ``global_grad_norm``) or, without it, that of ``grads``.
 
     Parameters and moments are dense fp32 tensors of one layout each, no two
-    of which share memory; gradients are fp32, bf16 or fp16, all of one type.
+    of which share memory; gradients do not share theirs and are fp32, bf16 or fp16, all of one type.
     ``step`` and ``lr`` are numbers of the host, so the call refuses to be
     captured into a graph, which would repeat them."""
     b1, b2 = (float(b) for b in betas)
@@ -102,7 +102,8 @@ def _reference_step(params, grads, exp_avgs, exp_avg_sqs, decay, step, lr,
     if len(devices) > 1:
         raise ValueError("fused_lamb_step: expected all tensors on one "
                          f"device, got {sorted(map(str, devices))}")
-    check_writable([*params, *exp_avgs, *exp_avg_sqs], "fused_lamb_step")
+    check_writable([*params, *exp_avgs, *exp_avg_sqs], "fused_lamb_step",
+                   read=grads)
     factor = 1.0
     if grad_norm is not None:
         factor = (max_grad_norm / (grad_norm.double() + 1e-6)) \

@@ -900,3 +900,19 @@ def test_clipping_views_of_negated_memory():
     ops.clip_grads_by_value_([view], 0.25)
     assert torch.equal(view.sign(), before.sign())
     assert view.abs().max() == 0.25
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_do_not_share_what_is_written(device):
+    _, (p, g, m, v) = make([64, 8], device)
+    before = [t.clone() for t in p + m + v]
+    wide = torch.ones(80, device=device)
+    for bad in ([p[0], g[1]], [g[0], m[1]], [m[0], g[1]], [g[0], v[0][3:11]],
+                [g[0], p[0][::8]]):
+        with pytest.raises(ValueError, match="memory"):
+            ops.fused_lamb_step(p, bad, m, v, step=1, lr=0.1)
+    for a, b in zip(p + m + v, before):
+        assert torch.equal(a, b)
+    # among each other they may: they are only read
+    ops.fused_lamb_step(p, [wide[:64], wide[60:68]], m, v, step=1, lr=0.1)
+    assert not torch.equal(p[1], before[1])
