@@ -916,3 +916,35 @@ def test_gradients_do_not_share_what_is_written(device):
     # among each other they may: they are only read
     ops.fused_lamb_step(p, [wide[:64], wide[60:68]], m, v, step=1, lr=0.1)
     assert not torch.equal(p[1], before[1])
+
+
+@pytest.mark.gpu
+def test_engine_replays_a_captured_step_that_clips(tmp_path, monkeypatch,
+                                                   capsys):
+    """--hip-graph with --clip-norm: the step is captured, not continued
+    eagerly, and each replay leaves gradients of the bound's norm."""
+    from byol_amd.engine import graph_step, trainer
+    from byol_amd.optim import build_optimizer
+    args = engine_args(tmp_path, "cuda", "--clip-norm", "0.001",
+                       "--channels-last", "--hip-graph")
+    torch.manual_seed(0)
+    loader, model, grapher = trainer.build_loader_model_grapher(args)
+    opt, _ = build_optimizer(model, args)
+    for group in opt.param_groups:
+        group["lr"] = 0.001  # past the warmup's zero
+    norms, replay = [], graph_step.GraphedTrainStep.replay
+
+    def watched(self, *inputs):
+        model.flat_space.flat_grads.fill_(9.0)  # not the last step's
+        out = replay(self, *inputs)
+        norms.append(ops.global_grad_norm([model.flat_space.flat_grads]))
+        return out
+    monkeypatch.setattr(graph_step.GraphedTrainStep, "replay", watched)
+    trainer.train(1, model, opt, loader.train_loader, grapher, args)
+    assert "capture failed" not in capsys.readouterr().out
+    assert len(norms) == 2  # of four minibatches the last two
+    # the norm and the factor are rounded, and each product
+    for norm in norms:
+        want = 0.001 / (1 + 1e-6 / 1e-3)  # at least, for norms above 0.001
+        assert want * (1 - 8 * E) <= norm.item() <= 0.001 * (1 + 8 * E)
+    assert torch.isfinite(model.flat_space.flat_params).all()
