@@ -247,18 +247,17 @@ __global__ __launch_bounds__(kSpanBlock) void grad_norm_partial_kernel(
     const SpanTable table, double* __restrict__ partial, int at,
     const NormEnd end) {
   __shared__ double scratch[kSpanBlock / WAVE_SIZE];
+  const int own = at + blockIdx.x;
+  if (threadIdx.x == 0)  // here its latency is hidden, at the end it is not
+    for (int i = own; i < end.cleared; i += end.all)
+      store_no_sum(end.clear + i);
   const double sum = chunk_sum<T, Reduce, true>(
       Chunk<const T>(table, blockIdx.x), scratch);
-  const int own = at + blockIdx.x;
   if (end.sums == nullptr) {
     if (threadIdx.x == 0) partial[own] = sum;
     return;
   }
-  if (threadIdx.x == 0) {
-    store_sum(end.sums + own, sum);
-    for (int i = own; i < end.cleared; i += end.all)
-      store_no_sum(end.clear + i);
-  }
+  if (threadIdx.x == 0) store_sum(end.sums + own, sum);
   if (own != end.all - 1) return;
   const uint64_t until = wall_clock64() + end.wait_ticks;
   for (;;) {
