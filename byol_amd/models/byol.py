@@ -66,7 +66,7 @@ class FlatParamSpace:
         self.flat_grads: Optional[torch.Tensor] = None
         # whether FlatDDP reduces flat_grads (it then holds all gradients)
         self.reduced = False
-        self._grad_views: List[torch.Tensor] = []
+        self._grad_views: List[Tuple[nn.Parameter, torch.Tensor]] = []
         self._homing = False
         # name -> (offset, numel, shape), in module.named_parameters() order
         self.layout: List[Tuple[str, int, int, torch.Size]] = []
@@ -90,7 +90,7 @@ class FlatParamSpace:
             view.copy_(p.detach())
             p.data = view
             p.grad = self.flat_grads[offset:offset + n].view(p.shape)
-            self._grad_views.append(p.grad)
+            self._grad_views.append((p, p.grad))
             offset += n
         return self.flat_params
 
@@ -135,7 +135,7 @@ class FlatParamSpace:
 
     def attach_grads(self) -> None:
         """Every parameter that has no gradient gets its view again."""
-        for p, view in zip(self.module.parameters(), self._grad_views):
+        for p, view in self._grad_views:
             if p.grad is None:
                 p.grad = view
 
@@ -143,15 +143,15 @@ class FlatParamSpace:
         """Zero the buffer and leave every ``p.grad`` at ``None``, until a
         backward pass reaches the parameter: its gradient is the view of the
         buffer then, as before.  So a parameter that no backward pass reaches
-        is seen to have no gradient, rather than one of zeros."""
+        is seen to have no gradient, rather than one of zeros.  (One that
+        ``torch.autograd.grad`` reaches counts as reached.)"""
         self.flat_grads.zero_()
-        params = list(self.module.parameters())
         if not self._homing:
-            for p, view in zip(params, self._grad_views):
+            for p, view in self._grad_views:
                 if p.requires_grad:
                     p.register_hook(self._make_homing_hook(p, view))
             self._homing = True
-        for p in params:
+        for p, _ in self._grad_views:
             p.grad = None
 
     @staticmethod

@@ -948,3 +948,26 @@ def test_engine_replays_a_captured_step_that_clips(tmp_path, monkeypatch,
         want = 0.001 / (1 + 1e-6 / 1e-3)  # at least, for norms above 0.001
         assert want * (1 - 8 * E) <= norm.item() <= 0.001 * (1 + 8 * E)
     assert torch.isfinite(model.flat_space.flat_params).all()
+
+
+def test_flat_space_drops_the_gradients_that_it_made():
+    """A parameter that the model gets later is none of the flat space's: it
+    does not shift the others' views."""
+    net, space, opt = flat_branches("cpu")
+    net.first = torch.nn.Linear(6, 6)
+    net._modules = {"first": net.first, **net._modules}  # comes first
+    x = torch.randn(8, 6)
+    for _ in range(2):
+        opt.zero_grad()
+        net(x).backward()
+        want = torch.autograd.grad(net(x), list(net.used.parameters()))
+        for p, g in zip(net.used.parameters(), want):
+            assert torch.allclose(p.grad, g)
+        opt.step()
+    space.flat_grads.fill_(2.0)
+    assert all((p.grad == 2).all() for p in net.used.parameters())
+    assert net.first.weight.grad is None
+    by_name = space.named_views(space.flat_grads)
+    for name, p in net.named_parameters():
+        if p.grad is not None:
+            assert p.grad.data_ptr() == by_name[name].data_ptr(), name
