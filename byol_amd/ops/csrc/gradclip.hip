@@ -5,8 +5,10 @@
 //
 // A block takes one chunk of one tensor and leaves one partial result; the last
 // block joins them in a fixed order, and the scaling pass reads the norm from
-// memory.  Nothing waits for the host, and as no result depends on the order in
-// which blocks run, a list gives the same bits every time.
+// memory.  Nothing waits for the host, and no result depends on the order in
+// which blocks run: a list in the same memory gives the same bits every time.
+// A captured graph joins in a launch of its own, with more threads and so in
+// another fixed order; that can change the last of the 64 bits.
 //
 // Squares are summed in 64 bits: the sum neither overflows for large fp32
 // gradients nor loses small ones.  All passes are bound by memory: the norm of
@@ -142,7 +144,7 @@ __device__ __forceinline__ double join_partials(int n, double* scratch,
   return red.template join<kThreads>(scratch);
 }
 
-// From a launch that has ended.
+// From launches that have ended.
 template <int kThreads>
 struct LoadPartials {
   const double* partial;
@@ -207,6 +209,10 @@ struct NormEnd {
   uint64_t wait_ticks;  // of 10 ns
   NormOut out;
 };
+
+// With `partial`, `at` and the 256 bytes that the compiler adds.
+static_assert(sizeof(SpanTable) + sizeof(NormEnd) + 16 + 256 <= 4096,
+              "kernel arguments are at most 4 KB");
 
 // A block's share of a norm: four packs of a thread at a time, or one (kWide
 // false), in the same order and so with the same bits.

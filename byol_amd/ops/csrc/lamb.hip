@@ -14,10 +14,11 @@
 //
 // The wait needs the other blocks to run at the same time, which nothing
 // guarantees: a tensor may have more chunks than fit the chip, and other work
-// may hold it.  So only the last chunks of a tensor wait, one for each CU (8.4 M
-// elements); a wait ends after a set time; and a block that does not wait, or
-// gave up, leaves its part of p to a second pass, which reads p, m and v again
-// and computes the same values.
+// may hold it.  So only the last chunks of a tensor wait: one for each CU (8.4 M
+// elements), or two of the smaller ones of a short list (4.2 M).  A wait ends
+// after a set time, and a block that does not wait, or gave up, leaves its part
+// of p to a second pass, which reads p, m and v again and computes the same
+// values.
 //
 // Bound by memory: 37 M parameters (ResNet-50 with its heads) take 202 us in
 // one launch, 5.1 TB/s, 76 M (ResNet-200) 373 us, 5.7 TB/s.  Two passes over all

@@ -47,7 +47,8 @@ constexpr int64_t kMaxSpanLen = int64_t(1) << 30;
 // flight (161 MB of fp16: 43 us with 1024, 38 us with 1536), more add sums to
 // join (46 MB of fp32, clipped: 26 us with 1536, 34 us with 8192).  Each
 // further table costs a launch that the one before has to drain for, about
-// 7 us: so a table holds as many spans as an argument of 4 KB can.
+// 7 us.  352 spans of 10 bytes leave 500 of the 4 KB that a kernel's arguments
+// may have for the others and for those that the compiler adds.
 constexpr int kMaxSpans = 352;
 constexpr int kTableChunks = 1536;
 

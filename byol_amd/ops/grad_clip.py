@@ -10,7 +10,9 @@ On GPU a list of any length is a few launches of the kernels in
 captured into a graph; sums are held in 64 bits and joined in a fixed order.
 Neighbouring views of one buffer (``FlatParamSpace.flat_grads``) are worked on
 as one tensor.  Elsewhere the same values come from elementary torch
-operations, the oracle of the tests.
+operations, the oracle of the tests.  In eager calls the norm's last block
+joins the others' sums while they come in, for which places are kept for the
+streams used last; in a captured graph a launch of its own joins them.
 
 Gradients are fp32, bf16 or fp16, types may differ within a list; strided
 tensors are taken as they are.  Tensors that are written must not overlap:

@@ -3,7 +3,8 @@
 The reference's LARS step runs ~6 ATen kernels per parameter tensor (~160
 tensors: two norm reductions, wd add, grad scale, momentum blend, param
 update — ``/root/reference/optimizers/lars.py:84-127`` + torch SGD).  Here the
-whole step is three HIP launches over the flat param/grad/momentum buffers:
+whole step is four HIP launches over the flat param/grad/momentum buffers, one
+that clears the accumulators and then:
 
 1. ``lars_norms``  — per-segment squared norms of p and (g + wd*p), one
    pass, block-per-chunk with atomics into per-segment accumulators;

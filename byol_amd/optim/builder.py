@@ -38,7 +38,7 @@ def build_lr_schedule(optimizer, args, last_epoch=-1):
 def build_optimizer(model, args, last_epoch=-1):
     """Returns (optimizer, scheduler).  When the model exposes a flat
     parameter space (``finalize()``d BYOL) the LARS wrapper gets it attached
-    so its step runs as three fused HIP kernel launches on GPU; LAMB gets it
+    so its step runs as four fused HIP kernel launches on GPU; LAMB gets it
     so its gradients stay in the buffer that FlatDDP reduces.  LAMB clips by
     ``--clip-norm`` inside its own step."""
     optim_map = {

@@ -15,7 +15,7 @@ MI355X fast path: when the model parameters live in a
 :class:`~byol_amd.models.byol.FlatParamSpace` and the inner optimizer is
 SGD+momentum, the whole step (per-tensor norms, weight decay, trust scaling,
 momentum, parameter update — the reference's ~160 tensors x ~6 ATen kernels)
-collapses into three HIP kernel launches over the flat buffers
+collapses into four HIP kernel launches over the flat buffers
 (:func:`byol_amd.ops.lars_step.fused_lars_momentum_step`).
 """
 
@@ -140,7 +140,7 @@ class LARS(Optimizer):
 
     def step(self, *args, **kwargs):
         # GPU + flat params + SGD/momentum inner: the whole multi-tensor
-        # step runs as three HIP kernel launches
+        # step runs as four HIP kernel launches
         if self._try_fused_step():
             return None
         self.apply_adaptive_lrs()
