@@ -68,6 +68,7 @@ class FlatParamSpace:
         self.reduced = False
         self._grad_views: List[Tuple[nn.Parameter, torch.Tensor]] = []
         self._homing = False
+        self._dropped: set = set()  # by index, since no gradient came back
         # name -> (offset, numel, shape), in module.named_parameters() order
         self.layout: List[Tuple[str, int, int, torch.Size]] = []
         self.numel = 0
@@ -134,10 +135,11 @@ class FlatParamSpace:
         self.flat_grads.zero_()
 
     def attach_grads(self) -> None:
-        """Every parameter that has no gradient gets its view again."""
+        """Every parameter that has no gradient gets its view again, with
+        zeros."""
         for p, view in self._grad_views:
             if p.grad is None:
-                p.grad = view
+                p.grad = view.zero_()
 
     def drop_grads(self) -> None:
         """Zero the buffer and leave every ``p.grad`` at ``None``, until a
@@ -147,18 +149,21 @@ class FlatParamSpace:
         ``torch.autograd.grad`` reaches counts as reached.)"""
         self.flat_grads.zero_()
         if not self._homing:
-            for p, view in self._grad_views:
+            for i, (p, _) in enumerate(self._grad_views):
                 if p.requires_grad:
-                    p.register_hook(self._make_homing_hook(p, view))
+                    p.register_hook(self._make_homing_hook(i))
             self._homing = True
         for p, _ in self._grad_views:
             p.grad = None
+        self._dropped = set(range(len(self._grad_views)))
 
-    @staticmethod
-    def _make_homing_hook(p, view):
+    def _make_homing_hook(self, i: int):
         def hook(_grad):  # runs before the gradient is accumulated
-            if p.grad is None:
+            # a gradient that others dropped left its values in the buffer
+            p, view = self._grad_views[i]
+            if i in self._dropped and p.grad is None:
                 p.grad = view
+            self._dropped.discard(i)
         return hook
 
     def grad_segments(self) -> List[Tuple[str, int, int]]:

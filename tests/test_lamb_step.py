@@ -971,3 +971,27 @@ def test_flat_space_drops_the_gradients_that_it_made():
     for name, p in net.named_parameters():
         if p.grad is not None:
             assert p.grad.data_ptr() == by_name[name].data_ptr(), name
+
+
+def test_flat_space_does_not_bring_old_gradients_back():
+    """Gradients that the model or another optimizer drops, which leaves their
+    values in the buffer, and FlatDDP around a model with such a buffer."""
+    net, space, opt = flat_branches("cpu")
+    xs = torch.randn(4, 8, 6)
+    opt.zero_grad()
+    net(xs[0]).backward()
+    opt.step()
+    params = list(net.used.parameters())
+    for x in xs[1:]:
+        net.zero_grad()
+        net(x).backward()
+        for p, g in zip(params, torch.autograd.grad(net(x), params)):
+            assert torch.allclose(p.grad, g)
+    opt.step()
+    opt.zero_grad()
+    net(xs[0]).backward()  # back in the buffer
+    space.flat_grads.fill_(2.0)
+    assert all((p.grad == 2).all() for p in params)
+    net.zero_grad()
+    space.attach_grads()
+    assert all((p.grad == 0).all() for p in net.parameters())
