@@ -41,7 +41,7 @@ namespace {
 // clipping 519, 489 and 462 us (in the order of the modules, see below).
 //
 // Short lists would leave CUs idle at that size: their blocks take 8192, all in
-// registers.  2 M elements take 22 us so and 33 us otherwise, 4.1 M 32 and 36,
+// registers.  2 M elements took 22 us so and 33 us otherwise, 4.1 M 32 and 36,
 // 5 M (where not all blocks of a tensor may wait any more) 48 and 38.
 constexpr int kLambBlock = 512;
 constexpr int kLongPacks = 16;  // packs of 4 elements of one thread

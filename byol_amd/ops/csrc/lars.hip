@@ -1,6 +1,7 @@
 // Fused multi-tensor LARS + SGD-momentum step over the flat parameter space.
 // Three launches, behind one that clears the sums, replace the reference's
-// ~6 ATen kernels x ~160 tensors (/root/reference/optimizers/lars.py:84-127 + torch SGD):
+// ~6 ATen kernels x ~160 tensors
+// (/root/reference/optimizers/lars.py:84-127 + torch SGD):
 //   1. lars_norms_kernel  — per-segment sum(p^2) and sum((g+wd*p)^2),
 //      block-per-chunk (chunk table precomputed host-side) with atomic
 //      accumulation into per-segment slots;

@@ -342,7 +342,8 @@ Norm norm_of(const Gradients& grads, bool inf, hipStream_t stream,
   if (places.sums == nullptr)
     launch_grad_norm_finish(parts, n, inf, full, rounded, stream);
   const hipError_t launched = hipGetLastError();
-  if (launched != hipSuccess && places.sums != nullptr) StreamSums::forget(stream);
+  if (launched != hipSuccess && places.sums != nullptr)
+    StreamSums::forget(stream);
   C10_HIP_CHECK(launched);
   return norm;
 }

@@ -47,7 +47,8 @@ def fused_lamb_step(params: Sequence[torch.Tensor],
     ``global_grad_norm``) or, without it, that of ``grads``.
 
     Parameters and moments are dense fp32 tensors of one layout each, no two
-    of which share memory; gradients do not share theirs and are fp32, bf16 or fp16, all of one type.
+    of which share memory; gradients do not share theirs and are fp32,
+    bf16 or fp16, all of one type.
     ``step`` and ``lr`` are numbers of the host, so the call refuses to be
     captured into a graph, which would repeat them."""
     b1, b2 = (float(b) for b in betas)

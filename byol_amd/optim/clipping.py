@@ -5,8 +5,8 @@ parameters that have one are handed to the fused operators of
 :mod:`byol_amd.ops.grad_clip`.  Those take fp32, bf16 and fp16 gradients on one
 device, no two of which reach into each other's memory.  By value, other
 gradients are bounded one by one in torch operations; by norm they are refused,
-and so are norms other than 2 and inf.  Under data parallelism call them after the
-gradients are synchronised (``FlatDDP.finish_grad_sync``): every replica then
+and so are norms other than 2 and inf.  Under data parallelism call them after
+the gradients are synchronised (``FlatDDP.finish_grad_sync``): every replica then
 computes the same norm from the same values, without another collective.
 """
 
